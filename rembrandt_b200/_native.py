@@ -75,10 +75,13 @@ _CUDA_SIGS = {
     "rb_categorical_loss": [vp, i32, i32, i32, vp, vp, f32, vp, vp, vp, vp, vp, vp, vp, i32, vp],
     "rb_softmax_ce": [vp, i32, i32, i32, i32, vp, vp, f32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp],
     # sgd_fused.cu
-    "rb_sgd_fused": [vp, vp, vp, vp, i64, f32, vp, f32, f32, f32, i32, i32, vp],
+    "rb_sgd_fused": [vp, vp, vp, vp, i64, f32, vp, f32, f32, f32, i32, i32, vp, vp],
     "rb_sgd_fused_grid": [vp, vp, vp, vp, i64, f32, vp, f32, f32, f32, i32, i32, i32, i32, vp],
     "rb_axpy_shadow": [vp, vp, vp, i64, f32, vp],
     "rb_axpby": [vp, vp, i64, f32, f32, vp],
+    # grad_clip.cu
+    "rb_grad_norm": [vp, vp, vp, i32, f32, f32, vp, vp, vp],
+    "rb_clip_grads": [vp, vp, vp, i32, f32, vp, vp],
     # input_pipeline.cu
     "rb_input_u8": [vp, vp, vp] + [i32] * 20 + [f32, f32, f32, vp, vp, u64, u32, vp, vp],
     "rb_var_input_u8": [vp, vp, vp, vp, i64] + [i32] * 14 + [f32, vp, f32, vp, vp, u64, u32, vp, vp],
@@ -91,6 +94,9 @@ _CUDA_SIGS = {
     "rb_bn_fwd_infer": [vp, i64, i32, i32, f32, vp, vp, vp, vp, vp, vp, vp, i32, vp],
     "rb_bn_fold": [vp, vp, i32, vp, vp],
     "rb_bn_bwd": [vp, vp, vp, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp],
+    # rms_norm.cu
+    "rb_rms_norm_fwd": [vp, vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, f32, i32, vp],
+    "rb_rms_norm_bwd": [vp, vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, vp],
 }
 
 

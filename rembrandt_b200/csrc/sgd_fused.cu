@@ -16,6 +16,7 @@ struct SgdArgs : SgdHyper {
   float* g;
   float* v;
   bf16* w16;   // optional
+  const float* clip;   // if given, clip[1] is a factor of the gradients (grad_clip.cu); where it is 0 they count as zeros
   long long n;
 };
 
@@ -23,12 +24,19 @@ __global__ void sgd_fused_kernel(const SgdArgs a) {
   pdl_prolog();
   SgdHyper h = a;
   if (h.lr_dev) h.lr = *h.lr_dev;
+  bool drop = false;
+  if (a.clip) {
+    const float coef = a.clip[1];
+    h.grad_scale *= coef;
+    drop = coef == 0.f;
+  }
   const long long n4 = a.n / 4;
   for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < n4;
        i += (long long)gridDim.x * blockDim.x) {
     float4 w = reinterpret_cast<float4*>(a.w)[i];
     float4 g = reinterpret_cast<float4*>(a.g)[i];
     float4 v = a.v ? reinterpret_cast<float4*>(a.v)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+    if (drop) g = make_float4(0.f, 0.f, 0.f, 0.f);
     sgd_elem(w.x, g.x, v.x, h);
     sgd_elem(w.y, g.y, v.y, h);
     sgd_elem(w.z, g.z, v.z, h);
@@ -47,7 +55,7 @@ __global__ void sgd_fused_kernel(const SgdArgs a) {
   // tail (n not a multiple of 4)
   for (long long i = n4 * 4 + blockIdx.x * (long long)blockDim.x + threadIdx.x; i < a.n;
        i += (long long)gridDim.x * blockDim.x) {
-    float w = a.w[i], g = a.g[i], v = a.v ? a.v[i] : 0.f;
+    float w = a.w[i], g = drop ? 0.f : a.g[i], v = a.v ? a.v[i] : 0.f;
     sgd_elem(w, g, v, h);
     if (a.phase & 3) a.w[i] = w;
     if (a.v && (a.phase & 1)) a.v[i] = v;
@@ -81,13 +89,13 @@ using namespace rb;
 
 extern "C" {
 
-// lr_dev: null, or one float on the device that is used instead of `lr`.
+// lr_dev: null, or one float on the device that is used instead of `lr`. clip: null, or what rb_grad_norm has written.
 int rb_sgd_fused(float* w, float* g, float* v, void* w16, long long n, float lr, const float* lr_dev, float mu, float l2,
-                 float grad_scale, int mode, int phase, cudaStream_t st) {
+                 float grad_scale, int mode, int phase, const float* clip, cudaStream_t st) {
   if (n <= 0) return 0;
   SgdArgs a;
   a.lr = lr; a.lr_dev = lr_dev; a.mu = mu; a.l2 = l2; a.grad_scale = grad_scale; a.mode = mode; a.phase = phase;
-  a.w = w; a.g = g; a.v = v; a.w16 = (bf16*)w16; a.n = n;
+  a.w = w; a.g = g; a.v = v; a.w16 = (bf16*)w16; a.clip = clip; a.n = n;
   // One block for every 256 x 4 values, whatever their number: blocks that start in order keep the seven streams of a sweep
   // within a few MB of one another, where 1184 blocks that step through the whole range spread them over all of it.
   // 62.4 M parameters: 279 -> 244 us (26 bytes each: 6.65 TB/s), 11.7 M: 55 -> 51 us, 1 M: 10 us both.
@@ -104,7 +112,7 @@ int rb_sgd_fused_grid(float* w, float* g, float* v, void* w16, long long n, floa
   if (blocks < 1 || threads < 32 || threads > 1024 || (threads & 31)) return -10;
   SgdArgs a;
   a.lr = lr; a.lr_dev = lr_dev; a.mu = mu; a.l2 = l2; a.grad_scale = grad_scale; a.mode = mode; a.phase = phase;
-  a.w = w; a.g = g; a.v = v; a.w16 = (bf16*)w16; a.n = n;
+  a.w = w; a.g = g; a.v = v; a.w16 = (bf16*)w16; a.clip = nullptr; a.n = n;
   const long long need = (n / 4 + threads - 1) / threads;
   if (need < blocks) blocks = need < 1 ? 1 : (int)need;
   launch_pdl(sgd_fused_kernel, blocks, threads, 0, st, a);

@@ -384,15 +384,136 @@ def rate_args(lr):
     return (0.0, ptr(lr)) if torch.is_tensor(lr) else (float(lr), None)
 
 
-def sgd_fused(w, g, v, w16, n, lr, mu, l2, grad_scale, mode, phase=7):
+def sgd_fused(w, g, v, w16, n, lr, mu, l2, grad_scale, mode, phase=7, clip=None):
+    """`clip`: what `grad_norm` has written (float32 [2]); the gradients count times its coefficient, and as zeros where that
+    is 0."""
+    if clip is not None:
+        _check_operand("clip", clip, torch.float32, 2, align=4)
     check(_native.cuda().rb_sgd_fused(ptr(w), ptr(g), ptr(v), ptr(w16), n, *rate_args(lr), mu, l2, grad_scale, mode, phase,
-                                      stream_handle()), "rb_sgd_fused")
+                                      ptr(clip), stream_handle()), "rb_sgd_fused")
 
 
 def sgd_fused_grid(w, g, v, w16, n, lr, mu, l2, grad_scale, mode, phase=7, blocks=296, threads=128):
     """The fused SGD sweep with an explicit grid (small blocks that co-reside with the GEMM CTAs)."""
     check(_native.cuda().rb_sgd_fused_grid(ptr(w), ptr(g), ptr(v), ptr(w16), n, *rate_args(lr), mu, l2, grad_scale, mode, phase,
                                            int(blocks), int(threads), stream_handle()), "rb_sgd_fused_grid")
+
+
+def _check_operand(name, t, dtype, n, align=16):
+    if not torch.is_tensor(t) or t.dtype != dtype or not t.is_contiguous() or t.numel() < n or t.data_ptr() % align:
+        what = f"{t.dtype} {tuple(t.shape)} at {t.data_ptr():#x}" if torch.is_tensor(t) else repr(t)
+        raise ValueError(f"{name} has to be {n} contiguous values of {dtype} on a {align}-byte boundary, not {what}")
+
+
+def _check_device(named):
+    """Every tensor of `named` (name, tensor or None) is on the device that the launch goes to."""
+    here = None
+    for name, t in named:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name} has to be on a GPU, not on {t.device}")
+        if here is None:
+            here = torch.cuda.current_device()
+        if t.get_device() != here:
+            raise ValueError(f"{name} is on {t.device}, but the current device is {here}")
+
+
+_GRAD_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+GRAD_NORM_SUMS = 1184       # 64-bit sums that `grad_norm` keeps between its launches
+
+
+def _is_dense(t):
+    """Whether the values of `t` fill one range of memory, in any order of its dimensions."""
+    if t.is_contiguous():
+        return True
+    step = 1
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda p: p[1]):
+        if stride != step:
+            return False
+        step *= size
+    return True
+
+
+class GradList:
+    """Gradients that a norm is taken over: float32, bfloat16 and float16 tensors of any sizes on one GPU, each filling one
+    range of memory and none of them overlapping. Their addresses are read when the list is made and it holds on to the
+    tensors, whose storage must not be exchanged (`set_`, `resize_`, `.data =`) as long as the list is used; a program whose
+    gradients are new tensors in every step gives `grad_norm` and `clip_grads` the tensors themselves."""
+
+    def __init__(self, tensors):
+        import ctypes as C_
+        self.tensors = tuple(tensors)
+        ends = []
+        for i, t in enumerate(self.tensors):
+            if not torch.is_tensor(t) or t.layout != torch.strided or t.dtype not in _GRAD_TYPES:
+                raise ValueError(f"gradient {i} has to be a float32, bfloat16 or float16 tensor, not "
+                                 f"{t.dtype if torch.is_tensor(t) else type(t).__name__}")
+            if not _is_dense(t):
+                raise ValueError(f"gradient {i} {tuple(t.shape)} with strides {t.stride()} leaves gaps in memory")
+            if t.numel():
+                ends.append((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), i))
+        ends.sort()
+        for (_, end, i), (at, _, j) in zip(ends, ends[1:]):
+            if at < end:
+                raise ValueError(f"gradients {i} and {j} overlap")
+        _check_same_device(self.tensors)
+        n = self.count = len(self.tensors)
+        self.device = self.tensors[0].device if n else None
+        self._at = (C_.c_void_p * n)(*(t.data_ptr() for t in self.tensors))
+        self._n = (C_.c_longlong * n)(*(t.numel() for t in self.tensors))
+        self._types = (C_.c_int * n)(*(_GRAD_TYPES[t.dtype] for t in self.tensors))
+        self.args = (C_.addressof(self._at), C_.addressof(self._n), C_.addressof(self._types), n)
+
+
+def _check_same_device(tensors):
+    for i, t in enumerate(tensors):
+        if not t.is_cuda:
+            raise ValueError(f"gradient {i} has to be on a GPU, not on {t.device}")
+        if t.device != tensors[0].device:
+            raise ValueError(f"gradient {i} is on {t.device}, the first on {tensors[0].device}")
+
+
+def grad_list(tensors):
+    """The gradients `tensors` as `grad_norm` and `clip_grads` take them, looked over once for many calls."""
+    return tensors if isinstance(tensors, GradList) else GradList(tensors)
+
+
+def grad_norm_scratch(device):
+    """Scratch of `grad_norm`, for calls that are ordered on one stream; graphs that may run at the same time have their own."""
+    return torch.zeros(GRAD_NORM_SUMS, dtype=torch.float64, device=device)
+
+
+def grad_norm(tensors, max_norm, out, ws, scale=1.0):
+    """out[0] = scale * (sum of the squares of all values of `tensors`)^1/2, their global norm; out[1] = the coefficient that
+    brings it down to `max_norm`: max_norm / out[0] where the norm is larger, 1 where it is not, 0 where it is no finite
+    float32. `out`: float32 [2]; `tensors`: a `GradList` or tensors that make one; `ws`: `grad_norm_scratch`. The sum is
+    taken in 64 bits and in the same order every time."""
+    tensors = grad_list(tensors)
+    max_norm, scale = float(max_norm), float(scale)
+    if not max_norm > 0.0:
+        raise ValueError(f"a largest norm has to be above 0, not {max_norm}")
+    _check_scale(scale)
+    _check_operand("out", out, torch.float32, 2, align=4)
+    _check_operand("scratch", ws, torch.float64, GRAD_NORM_SUMS)
+    _check_device((("out", out), ("scratch", ws), ("a gradient", tensors.tensors[0] if tensors.count else None)))
+    check(_native.cuda().rb_grad_norm(*tensors.args, scale, max_norm, ptr(out), ptr(ws), stream_handle()), "rb_grad_norm")
+
+
+def _check_scale(scale):
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"a scale of gradients has to be above 0 and finite, not {scale}")
+
+
+def clip_grads(tensors, out, scale=1.0):
+    """Every gradient of `tensors` times scale * out[1], rounded once to its own type; zeros where out[1] is 0, whatever they
+    hold. `out`: what `grad_norm` of the same tensors and scale has written."""
+    tensors = grad_list(tensors)
+    scale = float(scale)
+    _check_scale(scale)
+    _check_operand("out", out, torch.float32, 2, align=4)
+    _check_device((("out", out), ("a gradient", tensors.tensors[0] if tensors.count else None)))
+    check(_native.cuda().rb_clip_grads(*tensors.args, scale, ptr(out), stream_handle()), "rb_clip_grads")
 
 
 def axpy_shadow(w, v, w16, n, s):
@@ -504,3 +625,109 @@ def bn_bwd_ws(x, dy, y_relu, rows, C, c_valid, ws, mean, istd, gamma, dgamma, db
     _check_bn_scratch(ws, C)
     check(_native.cuda().rb_bn_bwd_ws(ptr(x), ptr(dy), ptr(y_relu), rows, C, c_valid, ptr(ws), ptr(mean), ptr(istd),
                                       ptr(gamma), ptr(dgamma), ptr(dbeta), ptr(dx), stream_handle()), "rb_bn_bwd_ws")
+
+
+# ------------------------------------------------------------------ normalisation over channels
+RMS_MAX_CHANNELS = 32768
+
+
+def _check_rms_shape(rows, C, c_valid):
+    if rows < 0 or C < 8 or C % 8 or C > RMS_MAX_CHANNELS or not 1 <= c_valid <= C or rows * C > 1 << 40:
+        raise ValueError(f"normalisation over channels takes a multiple of 8 channels up to {RMS_MAX_CHANNELS}, of which one at "
+                         f"least is live, not {rows} rows of {C} with {c_valid}")
+
+
+def _check_apart(name, out, named, same):
+    """`out` overlaps none of `named`, but may be all of one of them where `same`."""
+    lo = out.data_ptr()
+    hi = lo + out.numel() * out.element_size()
+    for other, t in named:
+        if t is None:
+            continue
+        at = t.data_ptr()
+        if at < hi and lo < at + t.numel() * t.element_size() and not (same and at == lo):
+            raise ValueError(f"{name} overlaps {other}")
+
+
+def _check_rms_eps(eps):
+    if not 2.0 ** -126 <= eps < float("inf"):
+        raise ValueError(f"an epsilon has to be a positive float32, not {eps}")
+
+
+def rms_norm_fwd(x, rows, C, c_valid, eps, gamma, y, rstd=None, residual=None, h=None, relu=False):
+    """h = x [+ residual], y = gamma * h / sqrt(mean of h^2 over the live channels + eps), and ReLU of it: a normalisation of every
+    row of [rows][C] by its own root mean square. `rstd` [rows] (float32, for `rms_norm_bwd`): the factor that stands for the
+    root; `h`: the sum, rounded to bf16 before it is normalised, whether it is stored or not. Channels from `c_valid` on count
+    as zeros and are written as such. `h` and `y` may each be `x` or `residual`."""
+    _check_rms_shape(rows, C, c_valid)
+    _check_rms_eps(eps)
+    n = rows * C
+    _check_operand("x", x, torch.bfloat16, n)
+    _check_operand("y", y, torch.bfloat16, n)
+    _check_operand("gamma", gamma, torch.float32, C)
+    inputs = (("x", x), ("residual", residual))
+    if residual is not None:
+        _check_operand("residual", residual, torch.bfloat16, n)
+    if h is not None:
+        _check_operand("h", h, torch.bfloat16, n)
+        _check_apart("h", h, inputs, True)
+        _check_apart("y", y, (("h", h),), False)
+    _check_apart("y", y, inputs, True)
+    if rstd is not None:
+        _check_operand("rstd", rstd, torch.float32, rows, align=4)
+    _check_device((*inputs, ("y", y), ("gamma", gamma), ("h", h), ("rstd", rstd)))
+    check(_native.cuda().rb_rms_norm_fwd(ptr(x), ptr(residual), ptr(h), ptr(y), None, None, ptr(rstd), ptr(gamma), rows, C, c_valid,
+                                         eps, int(relu), stream_handle()), "rb_rms_norm_fwd")
+
+
+def rms_norm_fwd_e4m3(x, rows, C, c_valid, eps, gamma, q, scales, residual=None, h=None, relu=False):
+    """`rms_norm_fwd` with its output in 8 bits: y is about q * scales[row], q e4m3 (torch.float8_e4m3fn) and scales float32
+    [rows], the largest |y| of the row / 448 (1 in a row of zeros, never below 2^-126). y is not rounded in between. A row that
+    holds a NaN or an infinity has a NaN as its scale and NaN codes. `q` overlaps no other operand; `h` may be `x` or `residual`."""
+    _check_rms_shape(rows, C, c_valid)
+    _check_rms_eps(eps)
+    n = rows * C
+    _check_operand("x", x, torch.bfloat16, n)
+    _check_operand("q", q, torch.float8_e4m3fn, n)
+    _check_operand("gamma", gamma, torch.float32, C)
+    _check_operand("scales", scales, torch.float32, rows, align=4)
+    inputs = (("x", x), ("residual", residual))
+    if residual is not None:
+        _check_operand("residual", residual, torch.bfloat16, n)
+    if h is not None:
+        _check_operand("h", h, torch.bfloat16, n)
+        _check_apart("h", h, inputs, True)
+    _check_apart("q", q, (*inputs, ("h", h)), False)
+    _check_device((*inputs, ("q", q), ("gamma", gamma), ("h", h), ("scales", scales)))
+    check(_native.cuda().rb_rms_norm_fwd(ptr(x), ptr(residual), ptr(h), None, ptr(q), ptr(scales), None, ptr(gamma), rows, C, c_valid,
+                                         eps, int(relu), stream_handle()), "rb_rms_norm_fwd")
+
+
+RMS_SCRATCH_ROWS = 592      # most blocks whose sums a backward pass joins
+
+
+def rms_norm_scratch(C, device):
+    """Scratch of `rms_norm_bwd` for up to C channels, for calls that are ordered on one stream; graphs that may run at the same
+    time have their own."""
+    return torch.zeros(RMS_SCRATCH_ROWS * C, dtype=torch.float32, device=device)
+
+
+def rms_norm_bwd(h, dy, rows, C, c_valid, rstd, gamma, dgamma, dx, ws, add=None, relu=False):
+    """Backward of `rms_norm_fwd`: dx = the delta of h (and so of x and of the residual), plus `add`, the delta that h has from
+    elsewhere; dgamma += its sum over the rows, in the same order every time. `dy` is the delta of y; with `relu` it is masked
+    here by the sign of y, which is worked out again. `h`: what was normalised (x where there was no residual). `dx` may be `h`,
+    `dy` or `add`; `ws`: `rms_norm_scratch`."""
+    _check_rms_shape(rows, C, c_valid)
+    n = rows * C
+    inputs = (("h", h), ("dy", dy), ("add", add))
+    for name, t in (*inputs, ("dx", dx)):
+        if t is not None or name != "add":
+            _check_operand(name, t, torch.bfloat16, n)
+    _check_operand("rstd", rstd, torch.float32, rows, align=4)
+    _check_operand("gamma", gamma, torch.float32, C)
+    _check_operand("dgamma", dgamma, torch.float32, C)
+    _check_operand("scratch", ws, torch.float32, RMS_SCRATCH_ROWS * C)
+    _check_apart("dx", dx, inputs, True)
+    _check_device((*inputs, ("dx", dx), ("rstd", rstd), ("gamma", gamma), ("dgamma", dgamma), ("scratch", ws)))
+    check(_native.cuda().rb_rms_norm_bwd(ptr(h), ptr(dy), ptr(add), ptr(dx), ptr(rstd), ptr(gamma), ptr(dgamma), ptr(ws), rows, C,
+                                         c_valid, int(relu), stream_handle()), "rb_rms_norm_bwd")
