@@ -5,9 +5,19 @@
 //             dx = r (g gamma - xhat m) [+ add],  dgamma += sum over rows of g xhat
 // Unlike a batch normalisation nothing here depends on the other samples of a batch, and there are no running statistics.
 // All sums are in fp32; h is the rounded sum, so that backward, which reads it, differentiates what forward computed.
+//
+// A row is read once and stays in registers between its sum and its output, which is all the traffic there is: 4 bytes a value
+// forward (8 with a residual that is kept, 3 into 8 bits), 6 backward (8 with `add`).
+//
+// How rows lie on threads. Vectors of 8 channels (16 bytes); vector v of a row belongs to lane v % lanes of the row's threads,
+// so that neighbouring lanes read neighbouring 16 bytes; a lane has V of them at most.
+//   narrow rows: L = 4 to 32 lanes of a warp hold one row, a warp 32 / L of them; sums are shuffles
+//   wide rows:   a block holds one row (L = 0)
 #include "launch.cuh"
 #include "common.cuh"
-#include <cuda_fp8.h>
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 namespace rb {
 
@@ -22,63 +32,265 @@ struct RmsArgs {
   const float* gamma;
   long long rows;
   int C, c_valid;
-  float eps;
+  float eps, inv_valid;
   int relu;
 };
+
+constexpr float E4M3_MAX = 448.f;
 
 __device__ __forceinline__ float max_nan(float a, float b) {   // as fmaxf, but NaN where either is
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-__device__ __forceinline__ float warp_max_nan(float v) {
+
+__device__ __forceinline__ float max_nan(float m, float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(m), "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_abs_nan(float m, float a, float b) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(m), "f"(a), "f"(b));
+  return d;
+}
+
+struct Plus {
+  __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+struct Most {
+  __device__ __forceinline__ float operator()(float a, float b) const { return max_nan(a, b); }
+};
+
+// v of all lanes of a row (L = 0: of the block), joined in the same order everywhere. `slots`: 16 floats of shared memory that
+// no other join uses between two barriers.
+template <int L, class F>
+__device__ __forceinline__ float join_row(float v, float* slots, F f) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = (L ? L : 32) >> 1; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if (L) return v;
+  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+  __syncthreads();
+  const int warps = blockDim.x >> 5;
+  v = slots[0];
+  for (int w = 1; w < warps; ++w) v = f(v, slots[w]);
   return v;
 }
 
-constexpr float E4M3_MAX = 448.f;
+// Two floats in one 64-bit register: one instruction multiplies or adds both. With it, constant lane counts, 32-bit offsets from
+// a base that is the block's and masks only where channels are dead, a vector of eight takes 100 instructions a warp instead
+// of 146 forward and 161 instead of 275 into 8 bits, which those kernels were bound by.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 both(float lo, float hi) {
+  f2 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ float2 parts(f2 a) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(a));
+  return d;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ f2 widen(uint32_t w) {   // two bf16 values
+  return both(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ uint32_t to_bf16(f2 a, bool relu = false) {
+  const float2 v = parts(a);
+  uint32_t d;
+  if (relu) asm("cvt.rn.relu.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(v.y), "f"(v.x));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(v.y), "f"(v.x));
+  return d;
+}
+__device__ __forceinline__ uint32_t to_e4m3(f2 a, f2 b, bool relu) {   // NaN stays NaN
+  const float2 v = parts(a), w = parts(b);
+  uint16_t lo, hi;
+  if (relu) {
+    asm("cvt.rn.satfinite.relu.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(v.y), "f"(v.x));
+    asm("cvt.rn.satfinite.relu.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(w.y), "f"(w.x));
+  } else {
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(v.y), "f"(v.x));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(w.y), "f"(w.x));
+  }
+  return lo | ((uint32_t)hi << 16);
+}
 
-// One warp per row; the row is read again for the output.
-__global__ void __launch_bounds__(128) rms_norm_kernel(const RmsArgs a) {
+// Eight bf16 values; `keep_live`: the first `live` of them, zeros behind.
+struct Vec8 {
+  uint32_t w[4];
+};
+__device__ __forceinline__ Vec8 load_vec(const bf16* p) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+  return Vec8{{v.x, v.y, v.z, v.w}};
+}
+__device__ __forceinline__ void store_vec(bf16* p, const Vec8& v) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+}
+__device__ __forceinline__ void keep_live(Vec8& v, int live) {
+  if (live >= 8) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v.w[i] = live > 2 * i + 1 ? v.w[i] : live == 2 * i + 1 ? v.w[i] & 0xffffu : 0u;
+}
+
+// The vectors of one thread: channel of the first, live channels (0 to 8; -1: behind the row's end), gamma (0 in dead ones).
+// Narrow rows lie on L lanes, wide ones (L = 0) on a block.
+template <int L, int V>
+struct RmsLane {
+  int rr, c0, live[V];    // row of the block
+  f2 gamma[V][4];
+  __device__ __forceinline__ int lanes() const { return L ? L : blockDim.x; }
+  __device__ __forceinline__ int next(int j) const { return j * lanes() * 8; }   // vector j behind the first, in channels
+  __device__ __forceinline__ RmsLane(const float* g, int C, int c_valid) {
+    rr = L ? threadIdx.x / (L ? L : 1) : 0;
+    c0 = (L ? threadIdx.x & (L - 1) : threadIdx.x) * 8;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int c = c0 + next(j);
+      live[j] = c >= C ? -1 : min(8, max(0, c_valid - c));
+      float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+      if (live[j] >= 0) {
+        lo = *reinterpret_cast<const float4*>(g + c);
+        hi = *reinterpret_cast<const float4*>(g + c + 4);
+      }
+      float all[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      if (c_valid < C) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) all[k] = k < live[j] ? all[k] : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) gamma[j][k] = both(all[2 * k], all[2 * k + 1]);
+    }
+  }
+};
+
+// Threads of a block: narrow rows 256 / L at a time, or one wide row.
+template <int L>
+struct RmsBlock {
+  enum { most = L ? 256 : 512, rows = L ? 256 / (L ? L : 1) : 1 };
+};
+
+// A block walks down the rows; the loads of its next rows are under way while it works on the present ones. There is one copy
+// of the work in the code, not one for each of several rows: short calls wait for their instructions.
+template <int L, int V, bool RES, bool Q8>
+__global__ void __launch_bounds__(RmsBlock<L>::most) rms_norm_kernel(const RmsArgs a) {
   pdl_prolog();
-  const int lane = threadIdx.x & 31;
-  const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (r >= a.rows) return;
-  const long long base = r * a.C;
-  auto h_at = [&](int c) {
-    if (c >= a.c_valid) return 0.f;
-    float v = bf2f(a.x[base + c]);
-    if (a.residual) v = bf2f(f2bf(v + bf2f(a.residual[base + c])));
-    return v;
+  __shared__ float slots[2][2][16];
+  const RmsLane<L, V> w(a.gamma, a.C, a.c_valid);
+  const unsigned off = (unsigned)(w.rr * a.C + w.c0);      // from the block's first row; less than 2^15
+  const bool dead = a.c_valid < a.C;
+  const long long step = (long long)gridDim.x * RmsBlock<L>::rows;
+  Vec8 hn[V], rn[RES ? V : 1];
+  auto fetch = [&](long long r0) {
+    const bf16 *x = a.x + r0 * a.C, *res = RES ? a.residual + r0 * a.C : nullptr;
+    const bool row = w.rr < a.rows - r0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (!row || w.live[j] < 0) { hn[j] = Vec8{{0, 0, 0, 0}}; if (RES) rn[j] = hn[j]; continue; }
+      hn[j] = load_vec(x + off + w.next(j));
+      if (RES) rn[j] = load_vec(res + off + w.next(j));
+    }
   };
-  float s = 0.f;
-  for (int c = lane; c < a.c_valid; c += 32) {
-    const float v = h_at(c);
-    s += v * v;
-  }
-  const float rstd = rsqrtf(warp_sum(s) / a.c_valid + a.eps);
-  if (a.rstd && lane == 0) a.rstd[r] = rstd;
-  auto y_of = [&](float h, int c) {
-    if (c >= a.c_valid) return 0.f;
-    const float y = h * rstd * a.gamma[c];
-    return a.relu && y <= 0.f ? 0.f : y;
-  };
-  float inv = 1.f;
-  if (a.q) {
-    float m = 0.f;
-    for (int c = lane; c < a.c_valid; c += 32) m = max_nan(m, fabsf(y_of(h_at(c), c)));
-    m = warp_max_nan(m);
-    // at least the smallest normal number, whose reciprocal is finite
-    const float scale = m == 0.f ? 1.f : max_nan(m / E4M3_MAX, 1.17549435e-38f);
-    inv = 1.f / scale;
-    if (lane == 0) a.scales[r] = scale;
-  }
-  for (int c = lane; c < a.C; c += 32) {
-    const float h = h_at(c), y = y_of(h, c);
-    if (a.h) a.h[base + c] = f2bf(h);
-    if (a.q) a.q[base + c] = __nv_cvt_float_to_fp8(y * inv, __NV_SATFINITE, __NV_E4M3);
-    else a.y[base + c] = f2bf(y);
+  int turn = 0;
+  long long r0 = (long long)blockIdx.x * RmsBlock<L>::rows;
+  fetch(r0);
+  for (; r0 < a.rows; r0 += step, turn ^= 1) {
+    const bool row = w.rr < a.rows - r0;
+    Vec8 hv[V];
+    f2 sum = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      hv[j] = hn[j];
+      if (RES) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) hv[j].w[k] = to_bf16(add2(widen(hv[j].w[k]), widen(rn[j].w[k])));
+      }
+      if (dead) keep_live(hv[j], w.live[j]);
+    }
+    fetch(r0 + step);
+    if (RES && a.h) {
+      bf16* h = a.h + r0 * a.C;
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (row && w.live[j] >= 0) store_vec(h + off + w.next(j), hv[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const f2 f = widen(hv[j].w[k]);
+        sum = fma2(f, f, sum);
+      }
+    const float s = join_row<L>(parts(sum).x + parts(sum).y, slots[turn][0], Plus());
+    const float rstd = rsqrtf(s * a.inv_valid + a.eps);
+    if (a.rstd && w.c0 == 0 && row) a.rstd[r0 + w.rr] = rstd;
+    // h r before gamma: neither product leaves fp32 where the output does not
+    const f2 rs = both(rstd, rstd);
+    f2 y[V][4];
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) y[j][k] = mul2(mul2(widen(hv[j].w[k]), rs), w.gamma[j][k]);
+    if (Q8) {
+      float m = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 t = parts(y[j][k]);
+          m = a.relu ? max_nan(m, t.x, t.y) : max_abs_nan(m, t.x, t.y);
+        }
+      m = join_row<L>(m, slots[turn][1], Most());
+      // at least the smallest normal number, whose reciprocal is finite
+      const float scale = m == 0.f ? 1.f : max_nan(m * (1.f / E4M3_MAX), 1.17549435e-38f);
+      const float inv = 1.f / scale;
+      if (w.c0 == 0 && row) a.scales[r0 + w.rr] = scale;
+      uint8_t* q = a.q + r0 * a.C;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if (w.live[j] < 0 || !row) continue;
+        uint2 o;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[j][k] = mul2(y[j][k], both(inv, inv));
+        if (a.relu) { o.x = to_e4m3(y[j][0], y[j][1], true); o.y = to_e4m3(y[j][2], y[j][3], true); }
+        else { o.x = to_e4m3(y[j][0], y[j][1], false); o.y = to_e4m3(y[j][2], y[j][3], false); }
+        if (dead && w.live[j] < 8) {   // a row of NaN has zeros there too
+          const unsigned long long keep = (1ull << (8 * w.live[j])) - 1;
+          o.x &= (uint32_t)keep;
+          o.y &= (uint32_t)(keep >> 32);
+        }
+        *reinterpret_cast<uint2*>(q + off + w.next(j)) = o;
+      }
+    } else {
+      bf16* to = a.y + r0 * a.C;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if (w.live[j] < 0 || !row) continue;
+        Vec8 o;
+        if (a.relu) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o.w[k] = to_bf16(y[j][k], true);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o.w[k] = to_bf16(y[j][k], false);
+        }
+        if (dead) keep_live(o, w.live[j]);
+        store_vec(to + off + w.next(j), o);
+      }
+    }
   }
 }
 
@@ -90,57 +302,160 @@ struct RmsBackArgs {
   const float* rstd;
   const float* gamma;
   float* dgamma;
+  float* sums;            // [blocks][C]: what each block has of dgamma
   long long rows;
   int C, c_valid;
+  float inv_valid;
   int relu;
 };
 
-__global__ void __launch_bounds__(128) rms_norm_back_kernel(const RmsBackArgs a) {
+// A thread has the same channels in all its rows and keeps their part of dgamma in registers; the block's rows are joined at the
+// end and the blocks by rms_dgamma_kernel, both in a fixed order (atomic additions would give other last bits every time).
+template <int L, int V, bool ADD>
+__global__ void __launch_bounds__(RmsBlock<L>::most) rms_norm_back_kernel(const RmsBackArgs a) {
   pdl_prolog();
-  const int lane = threadIdx.x & 31;
-  const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (r >= a.rows) return;
-  const long long base = r * a.C;
-  const float rstd = a.rstd[r];
-  float m = 0.f;
-  for (int c = lane; c < a.c_valid; c += 32) {
-    const float xhat = bf2f(a.h[base + c]) * rstd, gamma = a.gamma[c];
-    const float g = a.relu && !(gamma * xhat > 0.f) ? 0.f : bf2f(a.dy[base + c]);
-    m += g * gamma * xhat;
-  }
-  m = warp_sum(m) / a.c_valid;
-  for (int c = lane; c < a.C; c += 32) {
-    float d = 0.f;
-    if (c < a.c_valid) {
-      const float xhat = bf2f(a.h[base + c]) * rstd, gamma = a.gamma[c];
-      const float g = a.relu && !(gamma * xhat > 0.f) ? 0.f : bf2f(a.dy[base + c]);
-      d = rstd * (g * gamma - xhat * m);
-      if (a.add) d += bf2f(a.add[base + c]);
+  constexpr bool EARLY = L || V * (ADD ? 3 : 2) <= 6;   // registers hold the next rows as well
+  __shared__ float slots[2][16];
+  __shared__ __align__(16) float part[L ? V * 2048 : 4];
+  const RmsLane<L, V> w(a.gamma, a.C, a.c_valid);
+  const unsigned off = (unsigned)(w.rr * a.C + w.c0);
+  const bool dead = a.c_valid < a.C;
+  f2 acc[V][4];
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[j][k] = 0;
+  const long long step = (long long)gridDim.x * RmsBlock<L>::rows;
+  Vec8 hn[V], gn[V], an[ADD ? V : 1];
+  float rn;
+  auto fetch = [&](long long r0) {
+    const long long base = r0 * a.C;
+    const bf16 *h = a.h + base, *dy = a.dy + base, *add = ADD ? a.add + base : nullptr;
+    const bool row = w.rr < a.rows - r0;
+    rn = row ? a.rstd[r0 + w.rr] : 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (!row || w.live[j] < 0) { hn[j] = gn[j] = Vec8{{0, 0, 0, 0}}; continue; }
+      hn[j] = load_vec(h + off + w.next(j));
+      gn[j] = load_vec(dy + off + w.next(j));
+      if (ADD) an[j] = load_vec(add + off + w.next(j));
     }
-    a.dx[base + c] = f2bf(d);
+  };
+  int turn = 0;
+  long long r0 = (long long)blockIdx.x * RmsBlock<L>::rows;
+  if (EARLY) fetch(r0);
+  for (; r0 < a.rows; r0 += step, turn ^= 1) {
+    const bool row = w.rr < a.rows - r0;
+    if (!EARLY) fetch(r0);
+    Vec8 hv[V], gv[V], av[ADD ? V : 1];
+    const float rstd = rn;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      hv[j] = hn[j];
+      gv[j] = gn[j];
+      if (ADD) av[j] = an[j];
+    }
+    if (EARLY) fetch(r0 + step);
+    const f2 rs = both(rstd, rstd);
+    f2 sum = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (dead) {
+        keep_live(hv[j], w.live[j]);
+        keep_live(gv[j], w.live[j]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const f2 xhat = mul2(widen(hv[j].w[k]), rs), t = mul2(xhat, w.gamma[j][k]);
+        if (a.relu) {
+          const float2 p = parts(t);
+          uint32_t& g = gv[j].w[k];
+          g = (p.x > 0.f ? g & 0xffffu : 0u) | (p.y > 0.f ? g & 0xffff0000u : 0u);
+        }
+        const f2 g = widen(gv[j].w[k]);
+        acc[j][k] = fma2(g, xhat, acc[j][k]);
+        sum = fma2(g, t, sum);
+      }
+    }
+    // dx = r g gamma - h r^2 m
+    const float m = join_row<L>(parts(sum).x + parts(sum).y, slots[turn], Plus()) * a.inv_valid;
+    const float by = -(m * rstd) * rstd;
+    const f2 by2 = both(by, by);
+    bf16* dx = a.dx + r0 * a.C;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (w.live[j] < 0 || !row) continue;
+      Vec8 d;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const f2 gg = mul2(widen(gv[j].w[k]), w.gamma[j][k]);
+        const f2 t = ADD ? fma2(gg, rs, widen(av[j].w[k])) : mul2(gg, rs);
+        d.w[k] = to_bf16(fma2(widen(hv[j].w[k]), by2, t));
+      }
+      if (dead) keep_live(d, w.live[j]);
+      store_vec(dx + off + w.next(j), d);
+    }
+  }
+  float* mine = a.sums + (long long)blockIdx.x * a.C;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const float2 p0 = parts(acc[j][0]), p1 = parts(acc[j][1]), p2 = parts(acc[j][2]), p3 = parts(acc[j][3]);
+    // narrow: part[vector][row of the block][channel]
+    float4* to = reinterpret_cast<float4*>(L ? part + j * 2048 + threadIdx.x * 8 : mine + w.c0 + w.next(j));
+    if (L || w.live[j] >= 0) {
+      to[0] = make_float4(p0.x, p0.y, p1.x, p1.y);
+      to[1] = make_float4(p2.x, p2.y, p3.x, p3.y);
+    }
+  }
+  if (L) {
+    // 256 / width threads per channel add eight rows each, then the first of them what the others have
+    constexpr int width = L ? L * 8 : 256;
+    const int c = threadIdx.x & (width - 1), t = threadIdx.x / width;
+    float s[V];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      s[j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[j] += part[j * 2048 + (t * 8 + i) * width + c];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < V; ++j) part[j * 256 + threadIdx.x] = s[j];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (t == 0 && j * width + c < a.C) {
+#pragma unroll
+        for (int i = 1; i < 256 / width; ++i) s[j] += part[j * 256 + i * width + c];
+        mine[j * width + c] = s[j];
+      }
+    }
   }
 }
 
-// dgamma: one block per 32 channels, eight rows at a time, joined in a fixed order.
-__global__ void __launch_bounds__(256) rms_norm_dgamma_kernel(const RmsBackArgs a) {
+// dgamma += the blocks' sums: COLS channels to a block, 1024 / COLS of the sums at a time, joined in a fixed order.
+template <int COLS>
+__global__ void __launch_bounds__(1024) rms_dgamma_kernel(const float* __restrict__ sums, float* __restrict__ dgamma, int blocks,
+                                                          int C, int c_valid) {
   pdl_prolog();
-  __shared__ float part[8][33];
-  const int lane = threadIdx.x & 31, k = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  constexpr int AT_ONCE = 1024 / COLS;
+  __shared__ float part[32][COLS + 1];
+  const int k = threadIdx.x / COLS, c = blockIdx.x * COLS + threadIdx.x % COLS;
   float s = 0.f;
-  if (c < a.c_valid) {
-    const float gamma = a.gamma[c];
-    for (long long r = k; r < a.rows; r += 8) {
-      const float xhat = bf2f(a.h[r * a.C + c]) * a.rstd[r];
-      const float g = a.relu && !(gamma * xhat > 0.f) ? 0.f : bf2f(a.dy[r * a.C + c]);
-      s += g * xhat;
-    }
+  if (c < C) {
+#pragma unroll 5
+    for (int b = k; b < blocks; b += AT_ONCE) s += sums[(long long)b * C + c];
   }
-  part[k][lane] = s;
+#pragma unroll
+  for (int o = COLS; o < 32; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) < COLS) part[threadIdx.x >> 5][threadIdx.x & 31] = s;
   __syncthreads();
-  if (k == 0 && c < a.c_valid) {
-    for (int i = 1; i < 8; ++i) s += part[i][lane];
-    a.dgamma[c] += s;
-  }
+  // warp w has channel w of the block, a lane each of the 32 parts
+  const int ch = threadIdx.x >> 5;
+  if (ch >= COLS) return;
+  s = warp_sum(part[threadIdx.x & 31][ch]);
+  if ((threadIdx.x & 31) == 0 && blockIdx.x * COLS + ch < c_valid) dgamma[blockIdx.x * COLS + ch] += s;
 }
 
 }  // namespace rb
@@ -148,7 +463,50 @@ __global__ void __launch_bounds__(256) rms_norm_dgamma_kernel(const RmsBackArgs 
 using namespace rb;
 
 static bool rms_shape_ok(long long rows, int C, int c_valid) {
-  return rows >= 0 && C >= 8 && C % 8 == 0 && C <= 32768 && c_valid >= 1 && c_valid <= C && rows <= (1ll << 40) / C;
+  return rows >= 0 && C >= 8 && C % 8 == 0 && C <= 16384 && c_valid >= 1 && c_valid <= C && rows <= (1ll << 40) / C;
+}
+
+// Blocks of a kernel that an SM holds: grids are as large as fit at once, and the blocks walk down the rows.
+template <auto KERNEL>
+static int blocks_per_sm(int threads) {
+  static std::atomic<int> known[17];
+  int n = known[threads / 32].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, threads, 0) != cudaSuccess || n < 1) n = 1;
+    known[threads / 32].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+template <int n>
+using N = std::integral_constant<int, n>;
+
+// Calls go(L, V, threads) for rows of C channels. Up to 1024 channels: as few idle lanes as there can be with at most 4 vectors
+// each, and as many lanes where that is equal. Wider rows: one block, two vectors a thread from 2056 channels on, more where
+// 512 threads do not hold the row.
+template <class F>
+static void rms_cover(int C, F go) {
+  const int cg = C / 8;
+  if (cg > 128) {
+    const int V = cg <= 256 ? 1 : cg <= 1024 ? 2 : cg <= 1536 ? 3 : 4, threads = (ceil_div(cg, V) + 31) / 32 * 32;
+    if (V == 1) go(N<0>(), N<1>(), threads);
+    else if (V == 2) go(N<0>(), N<2>(), threads);
+    else if (V == 3) go(N<0>(), N<3>(), threads);
+    else go(N<0>(), N<4>(), threads);
+    return;
+  }
+  int lanes = 0, V = 0;
+  for (int l = 32; l >= 4; l >>= 1) {
+    const int v = ceil_div(cg, l);
+    if ((v <= 1 || v == 3 || l == 32) && v <= 4 && (!lanes || l * v < lanes * V)) { lanes = l; V = v; }
+  }
+  if (lanes == 4) V == 1 ? go(N<4>(), N<1>(), 256) : go(N<4>(), N<3>(), 256);
+  else if (lanes == 8) V == 1 ? go(N<8>(), N<1>(), 256) : go(N<8>(), N<3>(), 256);
+  else if (lanes == 16) V == 1 ? go(N<16>(), N<1>(), 256) : go(N<16>(), N<3>(), 256);
+  else if (V == 1) go(N<32>(), N<1>(), 256);
+  else if (V == 2) go(N<32>(), N<2>(), 256);
+  else if (V == 3) go(N<32>(), N<3>(), 256);
+  else go(N<32>(), N<4>(), 256);
 }
 
 extern "C" {
@@ -157,21 +515,48 @@ extern "C" {
 int rb_rms_norm_fwd(const void* x, const void* residual, void* h, void* y, void* q, float* scales, float* rstd,
                     const float* gamma, long long rows, int C, int c_valid, float eps, int relu, cudaStream_t st) {
   if (!rms_shape_ok(rows, C, c_valid) || (y != nullptr) == (q != nullptr) || (q && !scales)) return -10;
+  if (h && !residual) return -10;      // without a residual h is x
   if (rows == 0) return 0;
-  RmsArgs a{(const bf16*)x, (const bf16*)residual, (bf16*)h, (bf16*)y, (uint8_t*)q, scales, rstd, gamma, rows, C, c_valid,
-            eps, relu};
-  launch_pdl(rms_norm_kernel, (unsigned)((rows + 3) / 4), 128, 0, st, a);
+  const RmsArgs a{(const bf16*)x, (const bf16*)residual, (bf16*)h, (bf16*)y, (uint8_t*)q, scales, rstd, gamma, rows, C, c_valid,
+                  eps, 1.f / (float)c_valid, relu};
+  rms_cover(C, [&](auto lanes, auto vectors, int threads) {
+    constexpr int L = decltype(lanes)::value, V = decltype(vectors)::value;
+    auto go = [&](auto res, auto q8) {
+      constexpr auto kern = rms_norm_kernel<L, V, decltype(res)::value, decltype(q8)::value>;
+      const long long need = (rows + RmsBlock<L>::rows - 1) / RmsBlock<L>::rows, most = 148ll * blocks_per_sm<kern>(threads);
+      launch_pdl(kern, (unsigned)std::min(need, most), threads, 0, st, a);
+    };
+    if (residual) q ? go(std::true_type(), std::true_type()) : go(std::true_type(), std::false_type());
+    else q ? go(std::false_type(), std::true_type()) : go(std::false_type(), std::false_type());
+  });
   return RB_LAUNCH_OK();
 }
 
+// ws: 592 * C floats.
 int rb_rms_norm_bwd(const void* h, const void* dy, const void* add, void* dx, const float* rstd, const float* gamma,
                     float* dgamma, float* ws, long long rows, int C, int c_valid, int relu, cudaStream_t st) {
   if (!rms_shape_ok(rows, C, c_valid)) return -10;
   if (rows == 0) return 0;
-  RmsBackArgs a{(const bf16*)h, (const bf16*)dy, (const bf16*)add, (bf16*)dx, rstd, gamma, dgamma, rows, C, c_valid, relu};
-  // dgamma first: dx may be written over dy
-  launch_pdl(rms_norm_dgamma_kernel, (unsigned)((c_valid + 31) / 32), 256, 0, st, a);
-  launch_pdl(rms_norm_back_kernel, (unsigned)((rows + 3) / 4), 128, 0, st, a);
+  const RmsBackArgs a{(const bf16*)h, (const bf16*)dy, (const bf16*)add, (bf16*)dx, rstd, gamma, dgamma, ws, rows, C, c_valid,
+                      1.f / (float)c_valid, relu};
+  int blocks = 0;
+  rms_cover(C, [&](auto lanes, auto vectors, int threads) {
+    constexpr int L = decltype(lanes)::value, V = decltype(vectors)::value;
+    auto go = [&](auto with) {
+      constexpr auto kern = rms_norm_back_kernel<L, V, decltype(with)::value>;
+      const long long need = (rows + RmsBlock<L>::rows - 1) / RmsBlock<L>::rows;
+      blocks = (int)std::min(need, 148ll * std::min(4, blocks_per_sm<kern>(threads)));
+      launch_pdl(kern, blocks, threads, 0, st, a);
+    };
+    add ? go(std::true_type()) : go(std::false_type());
+  });
+  auto finish = [&](auto cols) {
+    constexpr int COLS = decltype(cols)::value;
+    launch_pdl(rms_dgamma_kernel<COLS>, (unsigned)ceil_div(c_valid, COLS), 1024, 0, st, (const float*)ws, dgamma, blocks, C, c_valid);
+  };
+  // eight channels a block while that leaves few blocks (92416 x 128: 16.2 us both launches against 17.0), 32 from there on
+  // (1500 x 9216: 23.0 against 27.3)
+  C <= 2048 ? finish(N<8>()) : finish(N<32>());
   return RB_LAUNCH_OK();
 }
 

@@ -628,7 +628,7 @@ def bn_bwd_ws(x, dy, y_relu, rows, C, c_valid, ws, mean, istd, gamma, dgamma, db
 
 
 # ------------------------------------------------------------------ normalisation over channels
-RMS_MAX_CHANNELS = 32768
+RMS_MAX_CHANNELS = 16384
 
 
 def _check_rms_shape(rows, C, c_valid):

@@ -41,7 +41,7 @@ def _formula(h, c_valid, gamma, relu, eps=EPS):
 
 
 SHAPES = [(1, 8, 8), (1, 8, 1), (3, 32, 16), (361, 128, 128), (37, 96, 80), (1000, 64, 64), (5, 160, 129), (2, 1024, 1000), (7, 1056, 1050),
-          (129, 4096, 4096), (33, 2080, 2055), (3, 32768, 32768), (2, 32736, 32730), (2, 8200, 8193), (4099, 32, 32), (700, 512, 500), (20000, 192, 192)]
+          (129, 4096, 4096), (33, 2080, 2055), (3, 16384, 16384), (2, 16352, 16350), (9, 768, 741), (2, 8200, 8193), (4099, 32, 32), (700, 512, 500), (20000, 192, 192)]
 
 
 @pytest.mark.parametrize("rows,C,c_valid", SHAPES)
@@ -269,7 +269,7 @@ def test_another_stream_and_a_captured_call():
 
 
 def test_more_than_two_to_the_31_values():
-    rows, C = 65540, 32768
+    rows, C = 131080, 16384
     x = torch.zeros((rows, C), device="cuda", dtype=torch.bfloat16)
     gen = torch.Generator(device="cuda").manual_seed(1)
     gamma, rstd = _gamma(gen, C, C), torch.empty(rows, device="cuda")
@@ -278,7 +278,7 @@ def test_more_than_two_to_the_31_values():
     y = torch.empty_like(x)
     K.rms_norm_fwd(x, rows, C, C, EPS, gamma, y, rstd=rstd)
     want, _ = _formula(last, C, gamma, False)
-    assert ((y[-4:].double() - want).abs() <= (2.0 ** -8 + 2 * _sum_error(C)) * want.abs()).all() and (y[:65536] == 0).all()
+    assert ((y[-4:].double() - want).abs() <= (2.0 ** -8 + 2 * _sum_error(C)) * want.abs()).all() and (y[:131072] == 0).all()
     dg = torch.zeros(C, device="cuda")
     K.rms_norm_bwd(x, x, rows, C, C, rstd, gamma, dg, y, K.rms_norm_scratch(C, "cuda"))
     dx, dgw, size, dg_size = _backward(last, last, C, rstd[-4:], gamma, False, None)
