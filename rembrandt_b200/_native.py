@@ -198,6 +198,8 @@ def host():
 def cuda():
     """The sm_100a kernel library (built on first use). Loading it needs no GPU; launching does."""
     global _CUDA
+    if _CUDA is not None:       # set once, with everything declared
+        return _CUDA
     with _LOCK:
         if _CUDA is None:
             path = _libdir() / "librembrandt_cuda.so"
@@ -255,4 +257,4 @@ def ptr(t):
 
 def stream_handle():
     import torch
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())

@@ -15,6 +15,7 @@
 //   wide rows:   a block holds one row (L = 0)
 #include "launch.cuh"
 #include "common.cuh"
+#include "f32x2.cuh"
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -77,35 +78,9 @@ __device__ __forceinline__ float join_row(float v, float* slots, F f) {
   return v;
 }
 
-// Two floats in one 64-bit register: one instruction multiplies or adds both. With it, constant lane counts, 32-bit offsets from
-// a base that is the block's and masks only where channels are dead, a vector of eight takes 100 instructions a warp instead
-// of 146 forward and 161 instead of 275 into 8 bits, which those kernels were bound by.
-typedef unsigned long long f2;
-__device__ __forceinline__ f2 both(float lo, float hi) {
-  f2 d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
-  return d;
-}
-__device__ __forceinline__ float2 parts(f2 a) {
-  float2 d;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(a));
-  return d;
-}
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-  f2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ f2 add2(f2 a, f2 b) {
-  f2 d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-  f2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
+// With two floats an instruction, constant lane counts, 32-bit offsets from a base that is the block's and masks only where channels
+// are dead, a vector of eight takes 100 instructions a warp instead of 146 forward and 161 instead of 275 into 8 bits, which
+// those kernels were bound by.
 __device__ __forceinline__ f2 widen(uint32_t w) {   // two bf16 values
   return both(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }

@@ -388,7 +388,7 @@ def sgd_fused(w, g, v, w16, n, lr, mu, l2, grad_scale, mode, phase=7, clip=None)
     """`clip`: what `grad_norm` has written (float32 [2]); the gradients count times its coefficient, and as zeros where that
     is 0."""
     if clip is not None:
-        _check_operand("clip", clip, torch.float32, 2, align=4)
+        _operand("clip", clip, torch.float32, 2, align=4)
     check(_native.cuda().rb_sgd_fused(ptr(w), ptr(g), ptr(v), ptr(w16), n, *rate_args(lr), mu, l2, grad_scale, mode, phase,
                                       ptr(clip), stream_handle()), "rb_sgd_fused")
 
@@ -399,28 +399,33 @@ def sgd_fused_grid(w, g, v, w16, n, lr, mu, l2, grad_scale, mode, phase=7, block
                                            int(blocks), int(threads), stream_handle()), "rb_sgd_fused_grid")
 
 
-def _check_operand(name, t, dtype, n, align=16):
-    if not torch.is_tensor(t) or t.dtype != dtype or not t.is_contiguous() or t.numel() < n or t.data_ptr() % align:
-        what = f"{t.dtype} {tuple(t.shape)} at {t.data_ptr():#x}" if torch.is_tensor(t) else repr(t)
-        raise ValueError(f"{name} has to be {n} contiguous values of {dtype} on a {align}-byte boundary, not {what}")
+def _operand(name, t, dtype, n, align=16):
+    """The address of `t`, which has to hold `n` values of `dtype` one after the other from a boundary on."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.numel() >= n and t.is_contiguous():
+        at = t.data_ptr()
+        if not at % align:
+            return at
+    what = f"{t.dtype} {tuple(t.shape)}" if isinstance(t, torch.Tensor) else repr(t)
+    raise ValueError(f"{name} has to be {n} contiguous values of {dtype} on a {align}-byte boundary, not {what}")
 
 
-def _check_device(named):
-    """Every tensor of `named` (name, tensor or None) is on the device that the launch goes to."""
-    here = None
-    for name, t in named:
+def _stream_of(tensors, names):
+    """The current stream of the current device, where all of `tensors` (or None) have to be."""
+    here = -1
+    for t, name in zip(tensors, names):
         if t is None:
             continue
         if not t.is_cuda:
             raise ValueError(f"{name} has to be on a GPU, not on {t.device}")
-        if here is None:
+        if here < 0:
             here = torch.cuda.current_device()
         if t.get_device() != here:
             raise ValueError(f"{name} is on {t.device}, but the current device is {here}")
+    return stream_handle()
 
 
 _GRAD_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-GRAD_NORM_SUMS = 1184       # 64-bit sums that `grad_norm` keeps between its launches
+GRAD_NORM_SUMS = 740       # 64-bit sums that `grad_norm` keeps between its launches
 
 
 def _is_dense(t):
@@ -459,7 +464,7 @@ class GradList:
                 raise ValueError(f"gradients {i} and {j} overlap")
         _check_same_device(self.tensors)
         n = self.count = len(self.tensors)
-        self.device = self.tensors[0].device if n else None
+        self.first = self.tensors[0] if n else None
         self._at = (C_.c_void_p * n)(*(t.data_ptr() for t in self.tensors))
         self._n = (C_.c_longlong * n)(*(t.numel() for t in self.tensors))
         self._types = (C_.c_int * n)(*(_GRAD_TYPES[t.dtype] for t in self.tensors))
@@ -489,15 +494,14 @@ def grad_norm(tensors, max_norm, out, ws, scale=1.0):
     brings it down to `max_norm`: max_norm / out[0] where the norm is larger, 1 where it is not, 0 where it is no finite
     float32. `out`: float32 [2]; `tensors`: a `GradList` or tensors that make one; `ws`: `grad_norm_scratch`. The sum is
     taken in 64 bits and in the same order every time."""
-    tensors = grad_list(tensors)
-    max_norm, scale = float(max_norm), float(scale)
+    tensors, max_norm, scale = grad_list(tensors), float(max_norm), float(scale)
     if not max_norm > 0.0:
         raise ValueError(f"a largest norm has to be above 0, not {max_norm}")
     _check_scale(scale)
-    _check_operand("out", out, torch.float32, 2, align=4)
-    _check_operand("scratch", ws, torch.float64, GRAD_NORM_SUMS)
-    _check_device((("out", out), ("scratch", ws), ("a gradient", tensors.tensors[0] if tensors.count else None)))
-    check(_native.cuda().rb_grad_norm(*tensors.args, scale, max_norm, ptr(out), ptr(ws), stream_handle()), "rb_grad_norm")
+    out_at = _operand("out", out, torch.float32, 2, 4)
+    ws_at = _operand("scratch", ws, torch.float64, GRAD_NORM_SUMS)
+    stream = _stream_of((out, ws, tensors.first), ("out", "scratch", "a gradient"))
+    check(_native.cuda().rb_grad_norm(*tensors.args, scale, max_norm, out_at, ws_at, stream), "rb_grad_norm")
 
 
 def _check_scale(scale):
@@ -508,12 +512,11 @@ def _check_scale(scale):
 def clip_grads(tensors, out, scale=1.0):
     """Every gradient of `tensors` times scale * out[1], rounded once to its own type; zeros where out[1] is 0, whatever they
     hold. `out`: what `grad_norm` of the same tensors and scale has written."""
-    tensors = grad_list(tensors)
-    scale = float(scale)
+    tensors, scale = grad_list(tensors), float(scale)
     _check_scale(scale)
-    _check_operand("out", out, torch.float32, 2, align=4)
-    _check_device((("out", out), ("a gradient", tensors.tensors[0] if tensors.count else None)))
-    check(_native.cuda().rb_clip_grads(*tensors.args, scale, ptr(out), stream_handle()), "rb_clip_grads")
+    out_at = _operand("out", out, torch.float32, 2, 4)
+    stream = _stream_of((out, tensors.first), ("out", "a gradient"))
+    check(_native.cuda().rb_clip_grads(*tensors.args, scale, out_at, stream), "rb_clip_grads")
 
 
 def axpy_shadow(w, v, w16, n, s):
@@ -637,21 +640,34 @@ def _check_rms_shape(rows, C, c_valid):
                          f"least is live, not {rows} rows of {C} with {c_valid}")
 
 
-def _check_apart(name, out, named, same):
-    """`out` overlaps none of `named`, but may be all of one of them where `same`."""
-    lo = out.data_ptr()
-    hi = lo + out.numel() * out.element_size()
-    for other, t in named:
-        if t is None:
-            continue
-        at = t.data_ptr()
-        if at < hi and lo < at + t.numel() * t.element_size() and not (same and at == lo):
-            raise ValueError(f"{name} overlaps {other}")
-
-
 def _check_rms_eps(eps):
     if not 2.0 ** -126 <= eps < float("inf"):
         raise ValueError(f"an epsilon has to be a positive float32, not {eps}")
+
+
+def _check_apart(name, at, size, other, other_at, other_size, same):
+    """The `size` bytes at `at` overlap none of another operand's, but may be those where `same`."""
+    if at < other_at + other_size and other_at < at + size and not (same and at == other_at):
+        raise ValueError(f"{name} overlaps {other}")
+
+
+def _rms_inputs(x, rows, C, c_valid, eps, gamma, residual, h):
+    """Checks what both forward forms take; the addresses of x, gamma, residual and h."""
+    _check_rms_shape(rows, C, c_valid)
+    _check_rms_eps(eps)
+    n = rows * C
+    x_at = _operand("x", x, torch.bfloat16, n)
+    gamma_at = _operand("gamma", gamma, torch.float32, C)
+    res_at = h_at = None
+    if residual is not None:
+        res_at = _operand("residual", residual, torch.bfloat16, n)
+    if h is not None:
+        if residual is None:
+            raise ValueError("h is x where there is no residual: it is not written")
+        h_at = _operand("h", h, torch.bfloat16, n)
+        _check_apart("h", h_at, 2 * n, "x", x_at, 2 * n, True)
+        _check_apart("h", h_at, 2 * n, "residual", res_at, 2 * n, True)
+    return x_at, gamma_at, res_at, h_at
 
 
 def rms_norm_fwd(x, rows, C, c_valid, eps, gamma, y, rstd=None, residual=None, h=None, relu=False):
@@ -659,48 +675,34 @@ def rms_norm_fwd(x, rows, C, c_valid, eps, gamma, y, rstd=None, residual=None, h
     row of [rows][C] by its own root mean square. `rstd` [rows] (float32, for `rms_norm_bwd`): the factor that stands for the
     root; `h`: the sum, rounded to bf16 before it is normalised, whether it is stored or not. Channels from `c_valid` on count
     as zeros and are written as such. `h` and `y` may each be `x` or `residual`."""
-    _check_rms_shape(rows, C, c_valid)
-    _check_rms_eps(eps)
+    x_at, gamma_at, res_at, h_at = _rms_inputs(x, rows, C, c_valid, eps, gamma, residual, h)
     n = rows * C
-    _check_operand("x", x, torch.bfloat16, n)
-    _check_operand("y", y, torch.bfloat16, n)
-    _check_operand("gamma", gamma, torch.float32, C)
-    inputs = (("x", x), ("residual", residual))
-    if residual is not None:
-        _check_operand("residual", residual, torch.bfloat16, n)
-    if h is not None:
-        _check_operand("h", h, torch.bfloat16, n)
-        _check_apart("h", h, inputs, True)
-        _check_apart("y", y, (("h", h),), False)
-    _check_apart("y", y, inputs, True)
-    if rstd is not None:
-        _check_operand("rstd", rstd, torch.float32, rows, align=4)
-    _check_device((*inputs, ("y", y), ("gamma", gamma), ("h", h), ("rstd", rstd)))
-    check(_native.cuda().rb_rms_norm_fwd(ptr(x), ptr(residual), ptr(h), ptr(y), None, None, ptr(rstd), ptr(gamma), rows, C, c_valid,
-                                         eps, int(relu), stream_handle()), "rb_rms_norm_fwd")
+    y_at = _operand("y", y, torch.bfloat16, n)
+    _check_apart("y", y_at, 2 * n, "x", x_at, 2 * n, True)
+    if res_at is not None:
+        _check_apart("y", y_at, 2 * n, "residual", res_at, 2 * n, True)
+    if h_at is not None:
+        _check_apart("y", y_at, 2 * n, "h", h_at, 2 * n, False)
+    rstd_at = None if rstd is None else _operand("rstd", rstd, torch.float32, rows, 4)
+    stream = _stream_of((x, gamma, y, residual, h, rstd), ("x", "gamma", "y", "residual", "h", "rstd"))
+    check(_native.cuda().rb_rms_norm_fwd(x_at, res_at, h_at, y_at, None, None, rstd_at, gamma_at, rows, C, c_valid, eps,
+                                         1 if relu else 0, stream), "rb_rms_norm_fwd")
 
 
 def rms_norm_fwd_e4m3(x, rows, C, c_valid, eps, gamma, q, scales, residual=None, h=None, relu=False):
     """`rms_norm_fwd` with its output in 8 bits: y is about q * scales[row], q e4m3 (torch.float8_e4m3fn) and scales float32
     [rows], the largest |y| of the row / 448 (1 in a row of zeros, never below 2^-126). y is not rounded in between. A row that
     holds a NaN or an infinity has a NaN as its scale and NaN codes. `q` overlaps no other operand; `h` may be `x` or `residual`."""
-    _check_rms_shape(rows, C, c_valid)
-    _check_rms_eps(eps)
+    x_at, gamma_at, res_at, h_at = _rms_inputs(x, rows, C, c_valid, eps, gamma, residual, h)
     n = rows * C
-    _check_operand("x", x, torch.bfloat16, n)
-    _check_operand("q", q, torch.float8_e4m3fn, n)
-    _check_operand("gamma", gamma, torch.float32, C)
-    _check_operand("scales", scales, torch.float32, rows, align=4)
-    inputs = (("x", x), ("residual", residual))
-    if residual is not None:
-        _check_operand("residual", residual, torch.bfloat16, n)
-    if h is not None:
-        _check_operand("h", h, torch.bfloat16, n)
-        _check_apart("h", h, inputs, True)
-    _check_apart("q", q, (*inputs, ("h", h)), False)
-    _check_device((*inputs, ("q", q), ("gamma", gamma), ("h", h), ("scales", scales)))
-    check(_native.cuda().rb_rms_norm_fwd(ptr(x), ptr(residual), ptr(h), None, ptr(q), ptr(scales), None, ptr(gamma), rows, C, c_valid,
-                                         eps, int(relu), stream_handle()), "rb_rms_norm_fwd")
+    q_at = _operand("q", q, torch.float8_e4m3fn, n)
+    scales_at = _operand("scales", scales, torch.float32, rows, 4)
+    for other, at in (("x", x_at), ("residual", res_at), ("h", h_at)):
+        if at is not None:
+            _check_apart("q", q_at, n, other, at, 2 * n, False)
+    stream = _stream_of((x, gamma, q, scales, residual, h), ("x", "gamma", "q", "scales", "residual", "h"))
+    check(_native.cuda().rb_rms_norm_fwd(x_at, res_at, h_at, None, q_at, scales_at, None, gamma_at, rows, C, c_valid, eps,
+                                         1 if relu else 0, stream), "rb_rms_norm_fwd")
 
 
 RMS_SCRATCH_ROWS = 592      # most blocks whose sums a backward pass joins
@@ -719,15 +721,17 @@ def rms_norm_bwd(h, dy, rows, C, c_valid, rstd, gamma, dgamma, dx, ws, add=None,
     `dy` or `add`; `ws`: `rms_norm_scratch`."""
     _check_rms_shape(rows, C, c_valid)
     n = rows * C
-    inputs = (("h", h), ("dy", dy), ("add", add))
-    for name, t in (*inputs, ("dx", dx)):
-        if t is not None or name != "add":
-            _check_operand(name, t, torch.bfloat16, n)
-    _check_operand("rstd", rstd, torch.float32, rows, align=4)
-    _check_operand("gamma", gamma, torch.float32, C)
-    _check_operand("dgamma", dgamma, torch.float32, C)
-    _check_operand("scratch", ws, torch.float32, RMS_SCRATCH_ROWS * C)
-    _check_apart("dx", dx, inputs, True)
-    _check_device((*inputs, ("dx", dx), ("rstd", rstd), ("gamma", gamma), ("dgamma", dgamma), ("scratch", ws)))
-    check(_native.cuda().rb_rms_norm_bwd(ptr(h), ptr(dy), ptr(add), ptr(dx), ptr(rstd), ptr(gamma), ptr(dgamma), ptr(ws), rows, C,
-                                         c_valid, int(relu), stream_handle()), "rb_rms_norm_bwd")
+    h_at = _operand("h", h, torch.bfloat16, n)
+    dy_at = _operand("dy", dy, torch.bfloat16, n)
+    dx_at = _operand("dx", dx, torch.bfloat16, n)
+    add_at = None if add is None else _operand("add", add, torch.bfloat16, n)
+    for other, at in (("h", h_at), ("dy", dy_at), ("add", add_at)):
+        if at is not None:
+            _check_apart("dx", dx_at, 2 * n, other, at, 2 * n, True)
+    rstd_at = _operand("rstd", rstd, torch.float32, rows, 4)
+    gamma_at = _operand("gamma", gamma, torch.float32, C)
+    dgamma_at = _operand("dgamma", dgamma, torch.float32, C, 4)
+    ws_at = _operand("scratch", ws, torch.float32, RMS_SCRATCH_ROWS * C)
+    stream = _stream_of((h, dy, dx, rstd, gamma, dgamma, ws, add), ("h", "dy", "dx", "rstd", "gamma", "dgamma", "scratch", "add"))
+    check(_native.cuda().rb_rms_norm_bwd(h_at, dy_at, add_at, dx_at, rstd_at, gamma_at, dgamma_at, ws_at, rows, C, c_valid,
+                                         1 if relu else 0, stream), "rb_rms_norm_bwd")
