@@ -36,6 +36,8 @@ def base_parser(desc, **defaults):
     ap.add_argument("--momentum", choices=sorted(MOMENTA), default=defaults.get("momentum", "nesterov"))
     ap.add_argument("--mu", type=float, default=defaults.get("mu", 0.9))
     ap.add_argument("--l2", type=float, default=defaults.get("l2", 5e-4))
+    ap.add_argument("--clip-norm", type=float, default=0.0,
+                    help="scale the gradients of an iteration down to this global norm where theirs is larger (0: never)")
     ap.add_argument("--iters", type=int, default=defaults.get("iters", 200))
     ap.add_argument("--display-iters", type=int, default=defaults.get("display_iters", 50))
     ap.add_argument("--checkpoint-iters", type=int, default=defaults.get("checkpoint_iters", 0))
@@ -160,6 +162,7 @@ def run_training(args, model_cfg, schedule: StepSizeSchedule = None, source=None
     minibatch = args.minibatch or args.batch
     opt = SgdOptConfig(minibatch_size=minibatch, step_size=schedule or StepSizeSchedule.constant(args.lr),
                        momentum=MOMENTA[args.momentum], mu=args.mu, l2_reg_coef=args.l2,
+                       clip_norm=args.clip_norm,
                        sync_order=ORDERS[args.sync_order] if args.sync_order else default_order(worker.name),
                        comm_interval=args.comm_interval, step_ref=StepSizeReference(args.step_ref),
                        checkpoint=CheckpointBehavior.KEEP if args.keep_averaged else CheckpointBehavior.DISCARD,

@@ -34,7 +34,10 @@ class StepEngine:
         self.net = net
         self.opt = opt
         self.comm = comm or NullComm()
-        self.stepper = SgdStepper(net, opt.momentum, opt.mu, opt.l2_reg_coef)
+        self.stepper = SgdStepper(net, opt.momentum, opt.mu, opt.l2_reg_coef, opt.clip_norm)
+        if opt.clip_norm and self._overlapped():
+            raise ValueError(f"{self.comm.name} updates parameters from inside backward, before the norm of all gradients is "
+                             "known: clip_norm needs an exchange that leaves the update to the end")
         self.is_cuda = net.is_cuda
         self.use_graph = use_graph and self.is_cuda
         self.accum = max(1, opt.minibatch_size // net.batch)   # batches per optimizer iteration
@@ -323,6 +326,12 @@ class StepEngine:
 
     def d2h_bytes_per_step(self) -> int:
         return 8 if self.is_cuda else 0
+
+    def grad_norm(self) -> Optional[float]:
+        """Global norm of the gradients of the last iteration, before they were clipped; None without `clip_norm`. Waits for
+        the step."""
+        self.synchronize()
+        return self.stepper.grad_norm()
 
     def set_lr(self, lr: float):
         self.lr = float(lr)

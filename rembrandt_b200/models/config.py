@@ -239,6 +239,34 @@ class ProjStackResConv2dCfg:
 
 
 @dataclass
+class RmsNormCfg:
+    """Normalisation of every position by the root mean square of its channels, with a scale per channel (at most 16384)."""
+    act: Act = Act.IDENTITY
+    epsilon: float = 1e-5
+    act_param: Optional[float] = None
+
+
+@dataclass
+class RmsConv2dCfg:
+    """Convolution without bias, normalised over the channels of each position: act(norm(conv(x)))."""
+    conv_size: int
+    conv_stride: int
+    conv_pad: int
+    out_channels: int
+    act: Act = Act.RECT
+    init_weights: ParamsInit = field(default_factory=lambda: ParamsInit.kaiming())
+    epsilon: float = 1e-5
+    act_param: Optional[float] = None
+
+
+@dataclass
+class RmsStackResConv2dCfg:
+    """Identity basic block, normalised over channels: relu(norm(x + conv3x3(relu(norm(conv3x3(x))))))."""
+    init_weights: ParamsInit = field(default_factory=lambda: ParamsInit.kaiming())
+    epsilon: float = 1e-5
+
+
+@dataclass
 class BotResConv2dCfg:
     """Bottleneck residual block (configuration only, as in the reference: conv.rs:3854-3886)."""
     bottleneck_channels: int = 0
@@ -337,6 +365,18 @@ class SequentialOperatorConfig:
 
     def proj_stack_res_conv2d(self, cfg: ProjStackResConv2dCfg, name=None):
         self.hidden_ops.append(NamedOp(self._name(name, "projres"), cfg))
+        return self
+
+    def rms_norm(self, cfg: RmsNormCfg, name=None):
+        self.hidden_ops.append(NamedOp(self._name(name, "rms"), cfg))
+        return self
+
+    def rms_conv2d(self, cfg: RmsConv2dCfg, name=None):
+        self.hidden_ops.append(NamedOp(self._name(name, "rmsconv"), cfg))
+        return self
+
+    def rms_stack_res_conv2d(self, cfg: RmsStackResConv2dCfg, name=None):
+        self.hidden_ops.append(NamedOp(self._name(name, "rmsres"), cfg))
         return self
 
     def bot_res_conv2d(self, cfg, name=None):

@@ -46,6 +46,9 @@ def _op_table():
         C.BNormConv2dCfg: R.BNormConv2dOp,
         C.StackResConv2dCfg: R.StackResConv2dOp,
         C.ProjStackResConv2dCfg: R.ProjStackResConv2dOp,
+        C.RmsConv2dCfg: R.RmsConv2dOp,
+        C.RmsStackResConv2dCfg: R.RmsStackResConv2dOp,
+        C.RmsNormCfg: R.RmsNormOp,
         C.SplitCfg: O.SplitOp,
         C.JoinCfg: O.JoinOp,
     }

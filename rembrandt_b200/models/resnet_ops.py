@@ -8,6 +8,9 @@ they are the convolution's epilogue (`FoldedNorms`; first layers of the special 
 normalised convolution: filter, scale, bias, running mean, running variance, in that order in the blob
 (conv.rs:379-406); only filter, scale and bias receive gradients; none of the normalisation parameters is
 L2-regularised (conv.rs:637-651).
+
+Beside them, without a counterpart there: the same convolution and residual block with a normalisation over the channels of
+each position (`_RmsConv`), which goes by no other sample and has no running statistics, and that normalisation alone.
 """
 from __future__ import annotations
 
@@ -43,7 +46,8 @@ class FoldedNorms:
     def of(net):
         # a first layer that reads whole windows or a space-to-depth image keeps its own launch: its plain output is what the
         # input's window is checked by
-        units = [u for op in net.ops if isinstance(op, _BlockBase) for u in op.units if not u.windowed and u.s2d is None]
+        units = [u for op in net.ops if isinstance(op, _BlockBase) for u in op.units
+                 if u.statistics and not u.windowed and u.s2d is None]
         return FoldedNorms(net, units) if units else None
 
     def compute(self):
@@ -52,6 +56,8 @@ class FoldedNorms:
 
 class _BnConv:
     """conv (no bias) -> batch norm [-> + residual] [-> ReLU], with its buffers and parameter segments."""
+
+    statistics = True    # normalises by statistics of the batch, or running ones that can be folded into the convolution
 
     def __init__(self, op: Op, tag, in_hw, in_c, in_cp, out_c, k, stride, pad, init, mov_avg, eps, s2d=None):
         """`s2d` = (f, r2, s2d_hw): the input operator hands over a space-to-depth'd image (a strided first layer on
@@ -83,14 +89,17 @@ class _BnConv:
         self.seg_rv = ParamSeg(n + ".run_var", (self.kp,), decay=False, trainable=False)
         self.segs = [self.seg_w, self.seg_g, self.seg_b, self.seg_rm, self.seg_rv]
 
+    def _alloc_norm(self, dev):
+        self.mean = torch.zeros(self.kp, device=dev)
+        self.istd = torch.ones(self.kp, device=dev)
+        self.sums = K.bn_scratch(self.kp, dev)
+
     def alloc(self, dx_forms=()):
         """`dx_forms`: the (addend, mask) combinations in which `backward` will be asked for the input's delta."""
         net = self.op.net
         dev, n = net.device, net.batch
         self.conv_out = torch.zeros((n, self.P, self.Q, self.kp), dtype=torch.bfloat16, device=dev)
-        self.mean = torch.zeros(self.kp, device=dev)
-        self.istd = torch.ones(self.kp, device=dev)
-        self.sums = K.bn_scratch(self.kp, dev)
+        self._alloc_norm(dev)
         self.dconv = torch.zeros_like(self.conv_out) if net.training_capable else None
         if self.windowed:
             self.windowed.alloc(n, dev, self.kp, False, False)
@@ -123,7 +132,10 @@ class _BnConv:
         else:
             K.conv_fprop_tc(x, n, self.gh, self.gw, self.cp, w16, self.ko, self.gk, self.gk, self.gs, self.gp, self.gp,
                             self.P, self.Q, self.conv_out, self.kp, n_valid=self.ko, n_store=self.kp)
-        rows = n * self.P * self.Q
+        self._norm_forward(n * self.P * self.Q, out, residual, relu, train)
+
+    def _norm_forward(self, rows, out, residual, relu, train):
+        net = self.op.net
         if train:
             # the factor comes from the device-side step counter, so that graph replays keep averaging correctly
             kind = 1 if self.mov_avg.kind == "cumulative" else 2
@@ -139,9 +151,7 @@ class _BnConv:
         add_masked: add is zero already where the mask is."""
         net = self.op.net
         n = net.batch
-        rows = n * self.P * self.Q
-        K.bn_bwd_ws(self.conv_out, dout, y_relu, rows, self.kp, self.ko, self.sums, self.mean, self.istd,
-                    self.v(self.seg_g), self.v(self.seg_g, "grads"), self.v(self.seg_b, "grads"), self.dconv)
+        self._norm_backward(n * self.P * self.Q, dout, y_relu)
         gw = self.v(self.seg_w, "grads")
         if self.windowed:
             self.windowed.backward(x, self.dconv, self.kp, gw)
@@ -162,6 +172,11 @@ class _BnConv:
             conv_dgrad(self.dconv, n, self.P, self.Q, self.kp, self.v(self.seg_w, "params16"), self.ko, self.cp, self.in_c,
                        self.k, self.s, self.p, self.h, self.w, dx, add=add, mask=mask, add_masked=add_masked,
                        wt=self.dgrad.wt if self.dgrad else None)
+
+    def _norm_backward(self, rows, dout, y_relu):
+        """self.dconv = delta of the convolution's output (and of what was added to it)."""
+        K.bn_bwd_ws(self.conv_out, dout, y_relu, rows, self.kp, self.ko, self.sums, self.mean, self.istd,
+                    self.v(self.seg_g), self.v(self.seg_g, "grads"), self.v(self.seg_b, "grads"), self.dconv)
 
     # ---- parameters
     def _w_int(self, w_oihw):
@@ -218,6 +233,74 @@ class _BnConv:
         return torch.relu(y) if relu else y
 
 
+def check_rms_norm(cp, eps):
+    """Refuses what the kernels of the normalisation over channels would refuse when they are first called."""
+    if cp > K.RMS_MAX_CHANNELS:
+        raise ValueError(f"a normalisation over channels takes at most {K.RMS_MAX_CHANNELS} channels, not {cp}")
+    if not 2.0 ** -126 <= eps < float("inf"):
+        raise ValueError(f"the epsilon of a normalisation has to be a positive float32, not {eps}")
+
+
+def rms_norm_ref(x, gamma, eps):
+    """x [N, C, ...] over the root of the mean of its squares along C, times gamma."""
+    shape = (1, -1) + (1,) * (x.dim() - 2)
+    return x * torch.rsqrt(x.square().mean(1, keepdim=True) + eps) * gamma.reshape(shape)
+
+
+class _RmsConv(_BnConv):
+    """conv (no bias) [-> + residual] -> normalisation over the channels of each position [-> ReLU]. The residual is added before
+    the normalisation, in its kernel: what is normalised is the sum, and both its parts get the same delta. Parameters: filter
+    and scale."""
+
+    statistics = False
+
+    def __init__(self, op: Op, tag, in_hw, in_c, in_cp, out_c, k, stride, pad, init, eps, s2d=None):
+        super().__init__(op, tag, in_hw, in_c, in_cp, out_c, k, stride, pad, init, None, eps, s2d=s2d)
+        check_rms_norm(self.kp, eps)
+        self.segs = [self.seg_w, self.seg_g]
+        self.seg_b = self.seg_rm = self.seg_rv = None
+
+    def _alloc_norm(self, dev):
+        self.rstd = torch.ones(self.op.net.batch * self.P * self.Q, device=dev)
+        self.scratch = K.rms_norm_scratch(self.kp, dev) if self.op.net.training_capable else None
+
+    def _norm_forward(self, rows, out, residual, relu, train):
+        # the sum that is normalised takes the place of the convolution's output, which nothing else reads
+        h = self.conv_out if train and residual is not None else None
+        K.rms_norm_fwd(self.conv_out, rows, self.kp, self.ko, self.eps, self.v(self.seg_g), out,
+                       rstd=self.rstd if train else None, residual=residual, h=h, relu=relu)
+
+    def _norm_backward(self, rows, dout, y_relu):
+        # `y_relu` needs no look: a ReLU's mask is worked out from the sum
+        K.rms_norm_bwd(self.conv_out, dout, rows, self.kp, self.ko, self.rstd, self.v(self.seg_g), self.v(self.seg_g, "grads"),
+                       self.dconv, self.scratch, relu=y_relu is not None)
+
+    def init_params(self, rng):
+        w = _draw(self.init, rng, (self.ko, self.in_c, self.k, self.k), self.k * self.k * self.in_c, self.ko)
+        self.v(self.seg_w).copy_(self._w_int(w))
+        self.v(self.seg_g).zero_()
+        self.v(self.seg_g)[: self.ko] = 1.0
+
+    def encode(self):
+        w = self._w_ref(self.v(self.seg_w).detach().float().cpu())
+        return [(w.reshape(-1), (self.k * self.k * self.in_c, self.ko)),
+                (self.v(self.seg_g).detach().float().cpu()[: self.ko].clone(), (1, self.ko))]
+
+    def decode(self, arrays):
+        w = torch.as_tensor(arrays[0][0]).reshape(self.ko, self.in_c, self.k, self.k)
+        self.v(self.seg_w).copy_(self._w_int(w))
+        self.v(self.seg_g).zero_()
+        self.v(self.seg_g)[: self.ko] = torch.as_tensor(arrays[1][0]).reshape(-1)
+        return 2
+
+    def ref(self, x, residual, relu, train, t):
+        y = F.conv2d(x, self._w_ref(self.v(self.seg_w)), None, stride=self.s, padding=self.p)
+        if residual is not None:
+            y = y + residual
+        y = rms_norm_ref(y, self.v(self.seg_g)[: self.ko], self.eps)
+        return torch.relu(y) if relu else y
+
+
 class _BlockBase(Op):
     has_params = True
     units = ()
@@ -243,6 +326,11 @@ class _BlockBase(Op):
 
 
 class BNormConv2dOp(_BlockBase):
+    def _unit(self, in_hw, in_c, in_cp, s2d):
+        cfg = self.cfg
+        return _BnConv(self, "conv", in_hw, in_c, in_cp, cfg.out_channels, cfg.conv_size, cfg.conv_stride, cfg.conv_pad,
+                       cfg.init_weights, cfg.bnorm_mov_avg, cfg.bnorm_epsilon, s2d=s2d)
+
     def setup(self, net, prev):
         super().setup(net, prev)
         cfg = self.cfg
@@ -255,8 +343,7 @@ class BNormConv2dOp(_BlockBase):
             f, r2, _out_hw, s2d_hw = layout.s2d_geometry(cfg.conv_size, cfg.conv_stride, h + 2 * cfg.conv_pad)
             prev.request_s2d(f, s2d_hw, cfg.conv_pad)
             s2d = (f, r2, s2d_hw)
-        self.u = _BnConv(self, "conv", (h, w), c, prev.out_cp, cfg.out_channels, cfg.conv_size, cfg.conv_stride,
-                         cfg.conv_pad, cfg.init_weights, cfg.bnorm_mov_avg, cfg.bnorm_epsilon, s2d=s2d)
+        self.u = self._unit((h, w), c, prev.out_cp, s2d)
         row_len = self.u.gk * self.u.gk * self.u.cp
         if type(prev) is DataOp and WindowedFirstLayer.fits(prev, cfg.conv_size, c, row_len, net.device):
             self.u.windowed = WindowedFirstLayer(prev, cfg.conv_size, cfg.conv_stride, cfg.conv_pad, self.u.P, self.u.Q,
@@ -385,3 +472,108 @@ class ProjStackResConv2dOp(_BlockBase):
         sc = self.u3.ref(x, None, False, train, t)
         a1 = self.u1.ref(x, None, True, train, t)
         return self.u2.ref(a1, sc, True, train, t)
+
+
+class RmsConv2dOp(BNormConv2dOp):
+    """out = act(norm(conv(x))), normalised over the channels of each position."""
+
+    def _unit(self, in_hw, in_c, in_cp, s2d):
+        cfg = self.cfg
+        return _RmsConv(self, "conv", in_hw, in_c, in_cp, cfg.out_channels, cfg.conv_size, cfg.conv_stride, cfg.conv_pad,
+                        cfg.init_weights, cfg.epsilon, s2d=s2d)
+
+
+class RmsStackResConv2dOp(_BlockBase):
+    """out = relu(norm2(x + conv3x3(relu(norm1(conv3x3(x))))))"""
+
+    def setup(self, net, prev):
+        super().setup(net, prev)
+        cfg = self.cfg
+        h, w, c = prev.out_hwc
+        mk = lambda tag: _RmsConv(self, tag, (h, w), c, prev.out_cp, c, 3, 1, 1, cfg.init_weights, cfg.epsilon)
+        self.u1, self.u2 = mk("conv1"), mk("conv2")
+        self.units = (self.u1, self.u2)
+        self.segs = self.u1.segs + self.u2.segs
+        self.out_hwc = (h, w, c)
+        self.out_cp = prev.out_cp
+        self.has_relu = True
+
+    def alloc(self):
+        super().alloc()
+        self.u1.alloc([(True, self.prev.has_relu)] if self.wants_prev_delta() else ())
+        self.u2.alloc([(False, True)])
+        self.a1 = torch.zeros_like(self.out)
+        self.da1 = torch.zeros_like(self.out) if self.net.training_capable else None
+
+    def forward(self, train, t):
+        x = self.prev.out
+        self.u1.forward(x, self.a1, None, True, train, t)
+        self.u2.forward(self.a1, self.out, x, True, train, t)
+
+    def backward(self):
+        x = self.prev.out
+        self.u2.backward(self.a1, self.dout, None, self.da1, self.a1)
+        if self.wants_prev_delta():
+            # the identity path's delta is that of the sum, which the second normalisation has left in `dconv`
+            self.u1.backward(x, self.da1, None, self.prev.dout, self.mask_src(), add=self.u2.dconv)
+        else:
+            self.u1.backward(x, self.da1, None, None, None)
+
+    def ref_forward(self, x, train, t):
+        a1 = self.u1.ref(x, None, True, train, t)
+        return self.u2.ref(a1, x, True, train, t)
+
+
+class RmsNormOp(Op):
+    """out = act(gamma * x / root mean square of x over its channels): after a convolution or an affine operator."""
+
+    has_params = True
+
+    def setup(self, net, prev):
+        super().setup(net, prev)
+        self.out_hwc, self.out_cp = prev.out_hwc, prev.out_cp
+        check_rms_norm(self.out_cp, self.cfg.epsilon)
+        self.seg_g = ParamSeg(self.name + ".scale", (self.out_cp,), decay=False)
+        self.segs = [self.seg_g]
+        self._setup_act(self.cfg.act, getattr(self.cfg, "act_param", None))
+
+    def alloc(self):
+        super().alloc()
+        rows = self._act_rows()
+        self.rstd = torch.ones(rows, device=self.net.device)
+        train = self.net.training_capable
+        self.scratch = K.rms_norm_scratch(self.out_cp, self.net.device) if train else None
+        # without a delta to hand on there is still the scale's gradient, whose kernel writes one
+        self.dx = torch.zeros_like(self.out) if train and not self.wants_prev_delta() else None
+
+    def init_params(self, rng):
+        self.view(self.seg_g).zero_()
+        self.view(self.seg_g)[: self.out_hwc[2]] = 1.0
+
+    def encode_params(self):
+        c = self.out_hwc[2]
+        return [(self.view(self.seg_g).detach().float().cpu()[:c].clone(), (1, c))]
+
+    def decode_params(self, arrays):
+        self.view(self.seg_g).zero_()
+        self.view(self.seg_g)[: self.out_hwc[2]] = torch.as_tensor(arrays[0][0]).reshape(-1)
+        return 1
+
+    def forward(self, train, t):
+        K.rms_norm_fwd(self.prev.out, self._act_rows(), self.out_cp, self.out_hwc[2], self.cfg.epsilon, self.view(self.seg_g),
+                       self.out, rstd=self.rstd if train else None, relu=self.has_relu)
+        self._act_forward()
+
+    def backward(self):
+        self._act_backward()
+        # the consumer already masked dout by this operator's ReLU
+        dx = self.dx if self.dx is not None else self.prev.dout
+        K.rms_norm_bwd(self.prev.out, self.dout, self._act_rows(), self.out_cp, self.out_hwc[2], self.rstd, self.view(self.seg_g),
+                       self.view(self.seg_g, "grads"), dx, self.scratch)
+        mask = self.mask_src()
+        if mask is not None and dx is not self.dx:
+            K.relu_mask(dx, mask, dx.numel())
+
+    def ref_forward(self, x, train, t):
+        y = rms_norm_ref(x, self.view(self.seg_g)[: self.out_hwc[2]], self.cfg.epsilon)
+        return self._ref_act(y)

@@ -9,8 +9,8 @@ the framework's headline benchmark is quoted on.
 from __future__ import annotations
 
 from .config import (Act, AffineCfg, BNormConv2dCfg, BNormMovingAverage, Conv2dCfg, Data3dCfg, DropoutCfg, LrnCfg,
-                     ParamsInit, Pool2dCfg, PoolKind, Preproc, ProjStackResConv2dCfg, SequentialOperatorConfig,
-                     SoftmaxKLLossCfg, StackResConv2dCfg)
+                     ParamsInit, Pool2dCfg, PoolKind, Preproc, ProjStackResConv2dCfg, RmsConv2dCfg,
+                     RmsStackResConv2dCfg, SequentialOperatorConfig, SoftmaxKLLossCfg, StackResConv2dCfg)
 
 # eigen-decomposition of ImageNet RGB covariance used for PCA lighting noise (AlexNet paper values)
 PCA_EIGVALS = (0.2175, 0.0188, 0.0045)
@@ -296,16 +296,24 @@ def go_policy_net(planes=32, channels=128, layers=6, num_classes=361):
     return cfg.softmax_kl_loss(SoftmaxKLLossCfg(num_classes))
 
 
-def go_policy_resnet(planes=32, channels=128, blocks=5, num_classes=361):
+def go_policy_resnet(planes=32, channels=128, blocks=5, num_classes=361, norm="batch"):
     """The residual move-prediction network the reference's Go tool trains (tools/train-gogod.rs:59-158): a
     batch-normalised 3x3 stem, `blocks` two-convolution residual blocks (moving-average factor 0.01, epsilon 1e-4)
-    and a 3x3 convolution to one plane, whose 19 x 19 outputs are the 361 move logits."""
+    and a 3x3 convolution to one plane, whose 19 x 19 outputs are the 361 move logits. norm="rms": normalised over the
+    channels of each point instead, so that a position's moves do not depend on the others of its batch."""
+    if norm not in ("batch", "rms"):
+        raise ValueError(f"unknown normalisation {norm!r}")
     k = ParamsInit.kaiming()
     cfg = SequentialOperatorConfig().data3d(Data3dCfg((19, 19, planes), normalize=True))
     mov = BNormMovingAverage("exponential", 0.01)
-    cfg.bnorm_conv2d(BNormConv2dCfg(3, 1, 1, channels, Act.RECT, k, mov, 1e-4), "stem")
-    for i in range(blocks):
-        cfg.stack_res_conv2d(StackResConv2dCfg(k, mov, 1e-4), f"res{i + 1}")
+    if norm == "rms":
+        cfg.rms_conv2d(RmsConv2dCfg(3, 1, 1, channels, Act.RECT, k, 1e-4), "stem")
+        for i in range(blocks):
+            cfg.rms_stack_res_conv2d(RmsStackResConv2dCfg(k, 1e-4), f"res{i + 1}")
+    else:
+        cfg.bnorm_conv2d(BNormConv2dCfg(3, 1, 1, channels, Act.RECT, k, mov, 1e-4), "stem")
+        for i in range(blocks):
+            cfg.stack_res_conv2d(StackResConv2dCfg(k, mov, 1e-4), f"res{i + 1}")
     cfg.conv2d(Conv2dCfg(3, 1, 1, 1, Act.IDENTITY, k), "move")
     return cfg.softmax_kl_loss(SoftmaxKLLossCfg(num_classes))
 

@@ -8,6 +8,7 @@ of the optimizer and the oracle the fused CUDA kernel is tested against.
 from __future__ import annotations
 
 import enum
+import math
 from dataclasses import dataclass, field
 from typing import Optional, Sequence
 
@@ -152,6 +153,7 @@ class SgdOptConfig:
     momentum: Momentum = Momentum.UPDATE
     mu: float = 0.9
     l2_reg_coef: float = 0.0
+    clip_norm: float = 0.0             # largest global norm of an iteration's gradients; 0 = they are taken as they are
     sync_order: SyncOrder = SyncOrder.SYNC_GRADS_THEN_STEP
     comm_interval: int = 1
     checkpoint: CheckpointBehavior = CheckpointBehavior.DISCARD
@@ -164,6 +166,14 @@ class SgdOptConfig:
 
 
 # ------------------------------------------------------------------------------------------ rules
+def clip_coefficient(norm: float, max_norm: float) -> float:
+    """The factor that brings gradients of this global norm down to `max_norm`: 1 where they are within it, 0 where the norm is
+    not finite (the step is then one with gradients of zeros). It multiplies the loss's gradients, before the L2 term."""
+    if not math.isfinite(norm):
+        return 0.0
+    return max_norm / norm if norm > max_norm else 1.0
+
+
 def reference_step(w, g, v, lr, mu, l2, grad_scale, mode, phase=7):
     """One optimizer step on plain tensors (modified in place, also returned).
 

@@ -4,21 +4,52 @@ On CUDA this is the fused one-pass kernel (csrc/sgd_fused.cu), launched once for
 once for the unregularised tail; on CPU it is ``reference_step``. ``phase`` lets the training loop split
 "accumulate into the momentum buffer" from "apply to the parameters" when a parameter exchange sits between
 the two (the reference's SyncParamsThenStep order, src/opt/sgd/new.rs:408-431).
+
+With `clip_norm` the gradients of all parameters are measured first (csrc/grad_clip.cu) and the sweep multiplies them by the
+coefficient, which it reads on the device: a captured step clips as an eager one does.
 """
 from __future__ import annotations
+
+import math
 
 import torch
 
 from ..ops import native_ops as K
-from .sgd import Momentum, reference_step
+from .sgd import Momentum, clip_coefficient, reference_step
 
 
 class SgdStepper:
-    def __init__(self, net, momentum: Momentum, mu: float, l2: float):
+    def __init__(self, net, momentum: Momentum, mu: float, l2: float, clip_norm: float = 0.0):
+        if not 0.0 <= clip_norm < math.inf:
+            raise ValueError(f"gradients are clipped to a norm above 0 (0: not at all), not {clip_norm}")
         self.net = net
         self.mode = int(momentum)
         self.mu = float(mu) if momentum != Momentum.ZERO else 0.0
         self.l2 = float(l2)
+        self.clip_norm = float(clip_norm)
+        # norm and coefficient of the present iteration: on the device, or as numbers
+        self.clip = torch.zeros(2, dtype=torch.float32, device=net.device) if net.is_cuda and self.clip_norm else None
+        self._clip_host = (0.0, 1.0)
+        self._clip_ws = K.grad_norm_scratch(net.device) if self.clip is not None else None
+        self._clip_list = None
+
+    def _measure(self, grad_scale):
+        """Norm and coefficient of all gradients, as they are now."""
+        net = self.net
+        if net.is_cuda:
+            if self._clip_list is None:
+                self._clip_list = K.grad_list([net.grads])
+            K.grad_norm(self._clip_list, self.clip_norm, self.clip, self._clip_ws, scale=grad_scale)
+        else:
+            norm = abs(grad_scale) * float(torch.linalg.vector_norm(net.grads.detach(), dtype=torch.float64))
+            self._clip_host = (norm, clip_coefficient(norm, self.clip_norm))
+
+    def grad_norm(self):
+        """Global norm of the gradients of the last iteration, before clipping; None where they are not clipped. Waits for the
+        device."""
+        if not self.clip_norm:
+            return None
+        return float(self.clip[0]) if self.clip is not None else self._clip_host[0]
 
     def _ranges(self, lo, hi):
         """Split [lo, hi) at the boundary between regularised and unregularised parameters."""
@@ -35,6 +66,14 @@ class SgdStepper:
         the sweep with small blocks (used when it runs beside backward)."""
         net = self.net
         hi = net.flat_len if hi is None else hi
+        clip = {}
+        if self.clip_norm:
+            if (lo, hi) != (0, net.flat_len):
+                raise ValueError("gradients are clipped by the norm of all of them: the sweep cannot take a part")
+            if phase & 1:        # a later phase of the iteration goes by the norm that this one has found
+                self._measure(grad_scale)
+            if net.is_cuda:
+                clip["clip"] = self.clip
         for a, b, l2 in self._ranges(lo, hi):
             n = b - a
             if net.is_cuda and grid is not None:
@@ -42,10 +81,13 @@ class SgdStepper:
                                  l2, grad_scale, self.mode, phase, grid[0], grid[1])
             elif net.is_cuda:
                 K.sgd_fused(net.params[a:b], net.grads[a:b], net.mom[a:b], net.params16[a:b], n, lr, self.mu, l2,
-                            grad_scale, self.mode, phase)
+                            grad_scale, self.mode, phase, **clip)
             else:
+                coef = self._clip_host[1] if self.clip_norm else 1.0
                 with torch.no_grad():
-                    reference_step(net.params[a:b], net.grads[a:b], net.mom[a:b], lr, self.mu, l2, grad_scale,
+                    if coef == 0.0:
+                        net.grads[a:b].zero_()
+                    reference_step(net.params[a:b], net.grads[a:b], net.mom[a:b], lr, self.mu, l2, grad_scale * coef,
                                    self.mode, phase)
 
     def nesterov_lookahead(self, sign: float = 1.0):

@@ -253,7 +253,8 @@ class SgdOpt:
                     disp_wall = time.time()
                     self._log(f"iter {t} epoch {epoch} step {eng.lr:.6g} loss {avg_loss:.4f} accuracy {acc:.4f} "
                               f"elapsed {wall:.3f}s" + (f" device {ips:.0f} images/s" if ips else "") +
-                              (f" exchange {bus:.1f} GB/s" if bus else ""))
+                              (f" exchange {bus:.1f} GB/s" if bus else "") +
+                              (f" gradient norm {eng.grad_norm():.4g}" if cfg.clip_norm else ""))
                     disp_loss = disp_correct = disp_samples = 0.0
 
                 if cfg.checkpoint_iters and t % cfg.checkpoint_iters == 0:
