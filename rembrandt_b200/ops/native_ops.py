@@ -401,7 +401,7 @@ def sgd_fused_grid(w, g, v, w16, n, lr, mu, l2, grad_scale, mode, phase=7, block
 
 def _operand(name, t, dtype, n, align=16):
     """The address of `t`, which has to hold `n` values of `dtype` one after the other from a boundary on."""
-    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.numel() >= n and t.is_contiguous():
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_contiguous() and t.numel() >= n:
         at = t.data_ptr()
         if not at % align:
             return at
@@ -409,19 +409,16 @@ def _operand(name, t, dtype, n, align=16):
     raise ValueError(f"{name} has to be {n} contiguous values of {dtype} on a {align}-byte boundary, not {what}")
 
 
-def _stream_of(tensors, names):
-    """The current stream of the current device, where all of `tensors` (or None) have to be."""
-    here = -1
-    for t, name in zip(tensors, names):
-        if t is None:
-            continue
-        if not t.is_cuda:
+def _stream_of(**tensors):
+    """The current stream of the current device, where all of the tensors (or None) have to be."""
+    devices = {t.get_device() for t in tensors.values() if t is not None}
+    here = devices.pop()
+    if not devices and here >= 0 and here == torch.cuda.current_device():
+        return stream_handle()
+    for name, t in tensors.items():
+        if t is not None and not t.is_cuda:
             raise ValueError(f"{name} has to be on a GPU, not on {t.device}")
-        if here < 0:
-            here = torch.cuda.current_device()
-        if t.get_device() != here:
-            raise ValueError(f"{name} is on {t.device}, but the current device is {here}")
-    return stream_handle()
+    raise ValueError("not all on the current device: " + ", ".join(f"{n} on {t.device}" for n, t in tensors.items() if t is not None))
 
 
 _GRAD_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -500,7 +497,7 @@ def grad_norm(tensors, max_norm, out, ws, scale=1.0):
     _check_scale(scale)
     out_at = _operand("out", out, torch.float32, 2, 4)
     ws_at = _operand("scratch", ws, torch.float64, GRAD_NORM_SUMS)
-    stream = _stream_of((out, ws, tensors.first), ("out", "scratch", "a gradient"))
+    stream = _stream_of(out=out, scratch=ws, gradient=tensors.first)
     check(_native.cuda().rb_grad_norm(*tensors.args, scale, max_norm, out_at, ws_at, stream), "rb_grad_norm")
 
 
@@ -515,7 +512,7 @@ def clip_grads(tensors, out, scale=1.0):
     tensors, scale = grad_list(tensors), float(scale)
     _check_scale(scale)
     out_at = _operand("out", out, torch.float32, 2, 4)
-    stream = _stream_of((out, tensors.first), ("out", "a gradient"))
+    stream = _stream_of(out=out, gradient=tensors.first)
     check(_native.cuda().rb_clip_grads(*tensors.args, scale, out_at, stream), "rb_clip_grads")
 
 
@@ -684,7 +681,7 @@ def rms_norm_fwd(x, rows, C, c_valid, eps, gamma, y, rstd=None, residual=None, h
     if h_at is not None:
         _check_apart("y", y_at, 2 * n, "h", h_at, 2 * n, False)
     rstd_at = None if rstd is None else _operand("rstd", rstd, torch.float32, rows, 4)
-    stream = _stream_of((x, gamma, y, residual, h, rstd), ("x", "gamma", "y", "residual", "h", "rstd"))
+    stream = _stream_of(x=x, gamma=gamma, y=y, residual=residual, h=h, rstd=rstd)
     check(_native.cuda().rb_rms_norm_fwd(x_at, res_at, h_at, y_at, None, None, rstd_at, gamma_at, rows, C, c_valid, eps,
                                          1 if relu else 0, stream), "rb_rms_norm_fwd")
 
@@ -700,7 +697,7 @@ def rms_norm_fwd_e4m3(x, rows, C, c_valid, eps, gamma, q, scales, residual=None,
     for other, at in (("x", x_at), ("residual", res_at), ("h", h_at)):
         if at is not None:
             _check_apart("q", q_at, n, other, at, 2 * n, False)
-    stream = _stream_of((x, gamma, q, scales, residual, h), ("x", "gamma", "q", "scales", "residual", "h"))
+    stream = _stream_of(x=x, gamma=gamma, q=q, scales=scales, residual=residual, h=h)
     check(_native.cuda().rb_rms_norm_fwd(x_at, res_at, h_at, None, q_at, scales_at, None, gamma_at, rows, C, c_valid, eps,
                                          1 if relu else 0, stream), "rb_rms_norm_fwd")
 
@@ -730,8 +727,8 @@ def rms_norm_bwd(h, dy, rows, C, c_valid, rstd, gamma, dgamma, dx, ws, add=None,
             _check_apart("dx", dx_at, 2 * n, other, at, 2 * n, True)
     rstd_at = _operand("rstd", rstd, torch.float32, rows, 4)
     gamma_at = _operand("gamma", gamma, torch.float32, C)
-    dgamma_at = _operand("dgamma", dgamma, torch.float32, C, 4)
+    dgamma_at = _operand("dgamma", dgamma, torch.float32, C)
     ws_at = _operand("scratch", ws, torch.float32, RMS_SCRATCH_ROWS * C)
-    stream = _stream_of((h, dy, dx, rstd, gamma, dgamma, ws, add), ("h", "dy", "dx", "rstd", "gamma", "dgamma", "scratch", "add"))
+    stream = _stream_of(h=h, dy=dy, dx=dx, rstd=rstd, gamma=gamma, dgamma=dgamma, scratch=ws, add=add)
     check(_native.cuda().rb_rms_norm_bwd(h_at, dy_at, add_at, dx_at, rstd_at, gamma_at, dgamma_at, ws_at, rows, C, c_valid,
                                          1 if relu else 0, stream), "rb_rms_norm_bwd")
