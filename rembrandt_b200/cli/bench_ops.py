@@ -46,7 +46,7 @@ def bf(*shape):
 
 
 def cases(batch):
-    """(name, function, algorithmic bytes) for the operators of AlexNet at the given batch."""
+    """(name, function, algorithmic bytes) for the operators of AlexNet at the given batch, and what other networks add."""
     out = []
     n = batch
     # ---- input: 3 x 227 x 227 bytes -> space-to-depth 57 x 57 x 64 bf16
@@ -96,6 +96,27 @@ def cases(batch):
     w, g, v = (torch.zeros(np_, device="cuda") for _ in range(3))
     w16 = torch.zeros(np_, dtype=torch.bfloat16, device="cuda")
     out.append(("sgd_fused_62M", lambda: K.sgd_fused(w, g, v, w16, np_, 0.01, 0.9, 5e-4, 1.0, 1), np_ * 26))
+    # ---- the same sweep with the gradients clipped by their norm, and clipping by itself (bf16, every value scaled)
+    clip, ws = torch.zeros(2, device="cuda"), K.grad_norm_scratch("cuda")
+    flat, half = K.grad_list([g]), K.grad_list([torch.ones(np_, device="cuda", dtype=torch.bfloat16)])
+
+    def clipped_step():
+        K.grad_norm(flat, 1.0, clip, ws)
+        K.sgd_fused(w, g, v, w16, np_, 0.01, 0.9, 5e-4, 1.0, 1, clip=clip)
+    out.append(("sgd_clipped_62M", clipped_step, np_ * 26))
+    out.append(("grad_norm_62M_bf16", lambda: K.grad_norm(half, 1.0, clip, ws), np_ * 2))
+    quarter = torch.tensor([4.0, 0.25], device="cuda")
+    out.append(("clip_grads_62M_bf16", lambda: K.clip_grads(half, quarter, scale=3.0), np_ * 4))
+    # ---- normalisation over channels on the Go network's layers (19 x 19 x 128, twice the batch)
+    rows, c = 2 * n * 361, 128
+    x, r, y, h = (bf(rows, c) for _ in range(4))
+    gamma, dgamma, rstd = torch.ones(c, device="cuda"), torch.zeros(c, device="cuda"), torch.ones(rows, device="cuda")
+    q, scales, nws = torch.empty((rows, c), device="cuda", dtype=torch.float8_e4m3fn), torch.empty(rows, device="cuda"), K.rms_norm_scratch(c, "cuda")
+    out.append(("rms_norm_fwd", lambda: K.rms_norm_fwd(x, rows, c, c, 1e-5, gamma, y, rstd=rstd, relu=True), rows * (c * 4 + 4)))
+    out.append(("rms_norm_fwd_residual", lambda: K.rms_norm_fwd(x, rows, c, c, 1e-5, gamma, y, rstd=rstd, residual=r, h=h, relu=True),
+                rows * (c * 8 + 4)))
+    out.append(("rms_norm_fwd_e4m3", lambda: K.rms_norm_fwd_e4m3(x, rows, c, c, 1e-5, gamma, q, scales, relu=True), rows * (c * 3 + 4)))
+    out.append(("rms_norm_bwd", lambda: K.rms_norm_bwd(x, r, rows, c, c, rstd, gamma, dgamma, y, nws, relu=True), rows * (c * 6 + 4)))
     return out
 
 

@@ -153,7 +153,6 @@ class SgdOptConfig:
     momentum: Momentum = Momentum.UPDATE
     mu: float = 0.9
     l2_reg_coef: float = 0.0
-    clip_norm: float = 0.0             # largest global norm of an iteration's gradients; 0 = they are taken as they are
     sync_order: SyncOrder = SyncOrder.SYNC_GRADS_THEN_STEP
     comm_interval: int = 1
     checkpoint: CheckpointBehavior = CheckpointBehavior.DISCARD
@@ -163,6 +162,7 @@ class SgdOptConfig:
     valid_iters: int = 0
     checkpoint_dir: Optional[str] = None
     max_iters: int = 0
+    clip_norm: float = 0.0             # largest global norm of an iteration's gradients; 0 = they are taken as they are
 
 
 # ------------------------------------------------------------------------------------------ rules

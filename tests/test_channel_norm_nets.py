@@ -213,7 +213,7 @@ def test_reference_path_gradients_are_differences():
     way = torch.randn(start.shape, generator=torch.Generator().manual_seed(2), dtype=torch.float64)
     way *= (start != 0)
     step = 1e-7
-    slope = (float(loss(start + step * way)) - float(loss(start - step * way))) / (2 * step)
+    slope = (loss(start + step * way).item() - loss(start - step * way).item()) / (2 * step)
     # central differences of step 1e-7 in 64 bits: 1e-16 / 1e-7 = 1e-9 of the loss, and 1e-14 of its third derivative; a ReLU
     # that changes sides within the step adds a part of its slope
     assert abs(slope - float((got * way).sum())) < 1e-5 * float((got * way).abs().sum())
@@ -340,6 +340,35 @@ def test_what_cannot_be_clipped_is_refused():
     with pytest.raises(ValueError, match="clip_norm"):
         StepEngine(net, opt, LocalOverlapComm())
     assert StepEngine(net, opt, NullComm()).stepper.clip_norm == 1.0
+
+
+def _two_ranks(rank, world):
+    import torch.distributed as dist
+    from rembrandt_b200.parallel.comm import AllreduceComm
+    torch.set_num_threads(1)
+    net = Net(zoo.mnist_fc1(), 8, device="cpu", seed=(3, 7))
+    opt = SgdOptConfig(minibatch_size=8, step_size=StepSizeSchedule.constant(0.5), momentum=Momentum.ZERO, mu=0.0, clip_norm=0.2)
+    eng = StepEngine(net, opt, AllreduceComm())
+    for i, (x, y) in enumerate(_batches(2 * 3, 8)):
+        if i % world != rank:        # every rank its own batches
+            continue
+        before = net.params.detach().clone()
+        eng.feed(x, y)
+        eng.step()
+        norm = eng.grad_norm()
+        moved = float((net.params.detach() - before).norm())
+        assert norm > 0.2 and abs(moved - 0.5 * 0.2) < 1e-5 * 0.1 + 2.0 ** -23 * float(before.norm())
+        both = torch.tensor([norm, -norm], dtype=torch.float64)
+        dist.all_reduce(both, op=dist.ReduceOp.MAX)
+        assert both[0] == norm and both[1] == -norm      # the norm of the averaged gradients, on every rank
+        first = net.params.detach().clone()
+        dist.broadcast(first, 0)
+        assert torch.equal(first, net.params.detach())
+
+
+def test_ranks_clip_what_they_have_averaged():
+    from cpu_ranks import run_ranks
+    run_ranks(2, _two_ranks)
 
 
 def test_clip_coefficient():

@@ -134,8 +134,9 @@ def test_the_same_norm_every_time_and_with_a_used_scratch():
     assert len(seen) == 1
 
 
-def test_another_stream_and_a_captured_call():
-    t = [torch.randn(300_000, device="cuda"), torch.randn(301, device="cuda").half()]
+@pytest.mark.parametrize("n", [300_000, 20_000])      # several launches, and one
+def test_another_stream_and_a_captured_call(n):
+    t = [torch.randn(n, device="cuda"), torch.randn(301, device="cuda").half()]
     first = [x.clone() for x in t]
     want = _norm(t)
     many, out, ws = K.grad_list(t), torch.zeros(2, device="cuda"), K.grad_norm_scratch("cuda")

@@ -211,6 +211,13 @@ def test_outputs_over_inputs(rows, C):
         yy = torch.empty_like(x) if y_at is None else both[y_at]
         K.rms_norm_fwd(both[0], rows, C, C, EPS, gamma, yy, rstd=rstd, residual=both[1], h=hh)
         assert torch.equal(yy, y) and torch.equal(hh, h)
+    q, scales = torch.empty((rows, C), device="cuda", dtype=torch.float8_e4m3fn), torch.empty(rows, device="cuda")
+    K.rms_norm_fwd_e4m3(x, rows, C, C, EPS, gamma, q, scales, residual=res)
+    for h_at in (0, 1):
+        both, q2, scales2 = [x.clone(), res.clone()], torch.empty_like(q), torch.empty_like(scales)
+        K.rms_norm_fwd_e4m3(both[0], rows, C, C, EPS, gamma, q2, scales2, residual=both[1], h=both[h_at])
+        assert torch.equal(both[h_at], h) and torch.equal(both[1 - h_at], (res, x)[h_at])
+        assert torch.equal(q2.float(), q.float()) and torch.equal(scales2, scales)
     for over in range(3):
         ins = [h.clone(), dy.clone(), add.clone()]
         dg2 = torch.zeros(C, device="cuda")
@@ -227,6 +234,31 @@ def test_no_rows():
     K.rms_norm_fwd_e4m3(x, 0, 64, 64, EPS, gamma, q, rstd)
     K.rms_norm_bwd(x, x, 0, 64, 64, rstd, gamma, dgamma, y, K.rms_norm_scratch(64, "cuda"))
     assert (y == 5).all() and rstd[0] == 5 and (dgamma == 3).all() and (q.float() == 1).all()
+
+
+def test_two_graphs_with_their_own_scratch_run_at_the_same_time():
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    rows, C = 30_000, 128
+    h, dy, gamma = _acts(gen, rows, C, C), _acts(gen, rows, C, C), _gamma(gen, C, C)
+    rstd = _formula(h, C, gamma, False)[1].float()
+    graphs = []
+    for scale in (1.0, 2.0):
+        dg, dx, ws, d = torch.zeros(C, device="cuda"), torch.empty_like(h), K.rms_norm_scratch(C, "cuda"), dy * scale
+        g, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=stream):
+            dg.zero_()
+            for _ in range(10):
+                K.rms_norm_bwd(h, d, rows, C, C, rstd, gamma, dg, dx, ws)
+        graphs.append((g, stream, dg, dx, d, ws))
+    for _ in range(5):
+        for g, stream, *_rest in graphs:
+            with torch.cuda.stream(stream):
+                g.replay()
+    torch.cuda.synchronize()
+    # deltas twice as large: every product and sum is twice as large, exactly
+    assert torch.equal(graphs[1][2], 2 * graphs[0][2]) and torch.equal(graphs[1][3], 2 * graphs[0][3])
+    assert graphs[0][2].abs().sum() > 0
 
 
 def test_another_stream_and_a_captured_call():
