@@ -469,15 +469,16 @@ template <int n>
 using N = std::integral_constant<int, n>;
 
 // Calls go(L, V, threads) for rows of C channels. Up to 1024 channels: as few idle lanes as there can be with at most 4 vectors
-// each, and as many lanes where that is equal. Wider rows: one block, two vectors a thread from 2056 channels on, more where
-// 512 threads do not hold the row.
+// each, and as many lanes where that is equal. Wider rows: one block with two vectors a thread, more where 512 threads do not hold
+// the row. Twice the threads with one vector each wait longer for one another (8000 x 2048: forward 14.8 us against 12.8, into 8
+// bits 19.0 against 13.5, backward 29.3 against 26.0), half of them with four keep less under way (6000 x 2560: backward 30.8
+// against 22.9).
 template <class F>
 static void rms_cover(int C, F go) {
   const int cg = C / 8;
   if (cg > 128) {
-    const int V = cg <= 256 ? 1 : cg <= 1024 ? 2 : cg <= 1536 ? 3 : 4, threads = (ceil_div(cg, V) + 31) / 32 * 32;
-    if (V == 1) go(N<0>(), N<1>(), threads);
-    else if (V == 2) go(N<0>(), N<2>(), threads);
+    const int V = cg <= 1024 ? 2 : cg <= 1536 ? 3 : 4, threads = (ceil_div(cg, V) + 31) / 32 * 32;
+    if (V == 2) go(N<0>(), N<2>(), threads);
     else if (V == 3) go(N<0>(), N<3>(), threads);
     else go(N<0>(), N<4>(), threads);
     return;
@@ -519,7 +520,7 @@ int rb_rms_norm_fwd(const void* x, const void* residual, void* h, void* y, void*
   return RB_LAUNCH_OK();
 }
 
-// ws: 592 * C floats.
+// ws: 592 * C floats; 1184 * C for 1032 to 2048 channels.
 int rb_rms_norm_bwd(const void* h, const void* dy, const void* add, void* dx, const float* rstd, const float* gamma,
                     float* dgamma, float* ws, long long rows, int C, int c_valid, int relu, cudaStream_t st) {
   if (!rms_shape_ok(rows, C, c_valid)) return -10;
@@ -532,9 +533,12 @@ int rb_rms_norm_bwd(const void* h, const void* dy, const void* add, void* dx, co
     auto go = [&](auto with) {
       constexpr auto kern = rms_norm_back_kernel<L, V, decltype(with)::value>;
       const long long need = (rows + RmsBlock<L>::rows - 1) / RmsBlock<L>::rows;
+      // a block for each of four resident ones, eight where they are small: fewer partial sums against more rows under way
+      // (12000 x 1280, 96 threads: 32.4 us with four, 24.2 with eight)
+      const int most = 148 * std::min(L || threads > 128 ? 4 : 8, blocks_per_sm<kern>(threads));
       // up to four times the rows that a block has at once, one block is as fast as several and a second launch (64 x 128: 2.9 us
       // against 3.0, 128 x 128: 4.2), but not where its vectors are many (32 x 512: 4.5 against 3.6)
-      blocks = need <= (L && V == 1 ? 4 : 1) ? 1 : (int)std::min(need, 148ll * std::min(4, blocks_per_sm<kern>(threads)));
+      blocks = need <= (L && V == 1 ? 4 : 1) ? 1 : (int)std::min(need, (long long)most);
       launch_pdl(kern, blocks, threads, 0, st, a);
     };
     add ? go(std::true_type()) : go(std::false_type());

@@ -702,13 +702,18 @@ def rms_norm_fwd_e4m3(x, rows, C, c_valid, eps, gamma, q, scales, residual=None,
                                          1 if relu else 0, stream), "rb_rms_norm_fwd")
 
 
-RMS_SCRATCH_ROWS = 592      # most blocks whose sums a backward pass joins
+RMS_SCRATCH_ROWS = 592      # most blocks whose sums a backward pass joins; twice as many for 1032 to 2048 channels
+
+
+def _rms_scratch_rows(C):
+    return RMS_SCRATCH_ROWS * (2 if 1024 < C <= 2048 else 1)
 
 
 def rms_norm_scratch(C, device):
     """Scratch of `rms_norm_bwd` for up to C channels, for calls that are ordered on one stream; graphs that may run at the same
     time have their own."""
-    return torch.zeros(RMS_SCRATCH_ROWS * C, dtype=torch.float32, device=device)
+    n = max(_rms_scratch_rows(c) * c for c in {C, min(C, 2048)})
+    return torch.zeros(n, dtype=torch.float32, device=device)
 
 
 def rms_norm_bwd(h, dy, rows, C, c_valid, rstd, gamma, dgamma, dx, ws, add=None, relu=False):
@@ -728,7 +733,7 @@ def rms_norm_bwd(h, dy, rows, C, c_valid, rstd, gamma, dgamma, dx, ws, add=None,
     rstd_at = _operand("rstd", rstd, torch.float32, rows, 4)
     gamma_at = _operand("gamma", gamma, torch.float32, C)
     dgamma_at = _operand("dgamma", dgamma, torch.float32, C)
-    ws_at = _operand("scratch", ws, torch.float32, RMS_SCRATCH_ROWS * C)
+    ws_at = _operand("scratch", ws, torch.float32, _rms_scratch_rows(C) * C)
     stream = _stream_of(h=h, dy=dy, dx=dx, rstd=rstd, gamma=gamma, dgamma=dgamma, scratch=ws, add=add)
     check(_native.cuda().rb_rms_norm_bwd(h_at, dy_at, add_at, dx_at, rstd_at, gamma_at, dgamma_at, ws_at, rows, C, c_valid,
                                          1 if relu else 0, stream), "rb_rms_norm_bwd")

@@ -86,6 +86,15 @@ def test_overlaps():
             _fwd(a | same)
 
 
+def test_a_scratch_serves_fewer_channels():
+    sizes = {C: K.rms_norm_scratch(C, "cpu").numel() for C in (8, 1024, 1032, 2048, 2056, 4096, 16384)}
+    assert list(sizes.values()) == sorted(sizes.values()) and all(n >= 592 * C for C, n in sizes.items())
+    a = _good(2, 2048)
+    for C, enough in ((1024, False), (2048, True), (2056, True), (4096, True)):
+        with pytest.raises(ValueError, match="GPU" if enough else "scratch"):
+            _bwd(a | {"ws": K.rms_norm_scratch(C, "cpu")})
+
+
 def test_gradients():
     for bad in (torch.zeros(4, dtype=torch.float64), torch.zeros(4, dtype=torch.int32), None, 3.0):
         with pytest.raises(ValueError, match="gradient 0"):

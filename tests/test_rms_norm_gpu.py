@@ -41,7 +41,7 @@ def _formula(h, c_valid, gamma, relu, eps=EPS):
 
 
 SHAPES = [(1, 8, 8), (1, 8, 1), (3, 32, 16), (361, 128, 128), (37, 96, 80), (1000, 64, 64), (5, 160, 129), (2, 1024, 1000), (7, 1056, 1050),
-          (129, 4096, 4096), (33, 2080, 2055), (3, 16384, 16384), (2, 16352, 16350), (9, 768, 741), (2, 8200, 8193), (1, 4104, 4099), (64, 128, 100), (65, 128, 100), (4, 1024, 999), (256, 32, 20), (4099, 32, 32), (700, 512, 500), (20000, 192, 192)]
+          (129, 4096, 4096), (2500, 1032, 1030), (1300, 2048, 2048), (33, 2080, 2055), (3, 16384, 16384), (2, 16352, 16350), (9, 768, 741), (2, 8200, 8193), (1, 4104, 4099), (64, 128, 100), (65, 128, 100), (4, 1024, 999), (256, 32, 20), (4099, 32, 32), (700, 512, 500), (20000, 192, 192)]
 
 
 @pytest.mark.parametrize("rows,C,c_valid", SHAPES)
