@@ -2,9 +2,9 @@
 //   out[0] = scale (sum over all values of all tensors of g^2)^1/2
 //   out[1] = min(1, max_norm / out[0]), the coefficient; 0 where out[0] is not finite
 //   clipping: g = scale out[1] g; zeros where out[1] is 0, whatever g holds
-// Squares are added in 64 bits, or in fp32 for the 16 or 32 values that a thread has at a time where that neither overflows nor loses any
-// (part_squares): no fp32 values are too large or too small for it. The sums of the blocks are joined in a fixed order, so that
-// the same gradients always have the same norm.
+// Squares are added in 64 bits, and in fp32 only among the 16 or 32 values that a thread has at a time, where that neither
+// overflows nor loses any (part_squares): no fp32 values are too large or too small for it. The sums of the blocks are joined in
+// a fixed order, so that the same gradients always have the same norm.
 //
 // Bound by memory: a norm reads each value once, clipping reads and writes it, and does nothing where the factor is 1. Measured
 // (us, and at the copy rate of 6.5 TB/s): norm of 62.4 M fp32 values 37.9 (38.2), of bf16 ones 21.6 (19.1); clipping 82 (76) and
@@ -19,7 +19,7 @@
 
 namespace rb {
 
-constexpr int NORM_BLOCKS = 740;        // most blocks of one launch: as many sums a scratch holds
+constexpr int NORM_BLOCKS = 740;         // most blocks of one launch: as many sums a scratch holds
 constexpr int VECTORS = 4;               // 16-byte vectors that a thread has under way
 constexpr int CHUNK = 256 * VECTORS;     // vectors of a tensor that a block takes at a time
 
@@ -144,8 +144,9 @@ __device__ __forceinline__ double block_sum(double s, double* part) {   // valid
   return s;
 }
 
-// Five blocks an SM, with four 16-byte loads under way per thread; with eight blocks the last round of chunks fills less of the
-// device (62.4 M fp32 values: 39.4 us). From the last chunk to the first: what is read last, and is still in the L2, is where the sweep that follows begins.
+// Five blocks an SM, with four 16-byte loads under way per thread: with eight, the last round of chunks fills less of the device
+// (62.4 M fp32 values: 39.4 us against 38.4). From the last chunk to the first: what is read last, and is still in the L2, is where
+// the sweep that follows begins.
 // `again`: a later launch of the same norm adds to what the first has left.
 template <int TENSORS>
 __global__ void __launch_bounds__(256) grad_squares_kernel(const __grid_constant__ GradTable<TENSORS> t, double* __restrict__ ws,

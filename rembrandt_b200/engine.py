@@ -37,7 +37,7 @@ class StepEngine:
         self.stepper = SgdStepper(net, opt.momentum, opt.mu, opt.l2_reg_coef, opt.clip_norm)
         if opt.clip_norm and self._overlapped():
             raise ValueError(f"{self.comm.name} updates parameters from inside backward, before the norm of all gradients is "
-                             "known: clip_norm needs an exchange that leaves the update to the end")
+                             "known: clip_norm needs an exchange that leaves the update to the end, such as allreduce")
         self.is_cuda = net.is_cuda
         self.use_graph = use_graph and self.is_cuda
         self.accum = max(1, opt.minibatch_size // net.batch)   # batches per optimizer iteration

@@ -492,8 +492,8 @@ def grad_norm(tensors, max_norm, out, ws, scale=1.0):
     float32. `out`: float32 [2]; `tensors`: a `GradList` or tensors that make one; `ws`: `grad_norm_scratch`. The sum is
     taken in 64 bits and in the same order every time."""
     tensors, max_norm, scale = grad_list(tensors), float(max_norm), float(scale)
-    if not max_norm > 0.0:
-        raise ValueError(f"a largest norm has to be above 0, not {max_norm}")
+    if not max_norm >= 2.0 ** -149:
+        raise ValueError(f"a largest norm has to be a float32 above 0, not {max_norm}")
     _check_scale(scale)
     out_at = _operand("out", out, torch.float32, 2, 4)
     ws_at = _operand("scratch", ws, torch.float64, GRAD_NORM_SUMS)
@@ -502,8 +502,8 @@ def grad_norm(tensors, max_norm, out, ws, scale=1.0):
 
 
 def _check_scale(scale):
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"a scale of gradients has to be above 0 and finite, not {scale}")
+    if not 2.0 ** -126 <= scale < 2.0 ** 128:
+        raise ValueError(f"a scale of gradients has to be a positive float32, not {scale}")
 
 
 def clip_grads(tensors, out, scale=1.0):
@@ -671,7 +671,8 @@ def rms_norm_fwd(x, rows, C, c_valid, eps, gamma, y, rstd=None, residual=None, h
     """h = x [+ residual], y = gamma * h / sqrt(mean of h^2 over the live channels + eps), and ReLU of it: a normalisation of every
     row of [rows][C] by its own root mean square. `rstd` [rows] (float32, for `rms_norm_bwd`): the factor that stands for the
     root; `h`: the sum, rounded to bf16 before it is normalised, whether it is stored or not. Channels from `c_valid` on count
-    as zeros and are written as such. `h` and `y` may each be `x` or `residual`."""
+    as zeros and are written as such. A row whose squares add up to more than float32 holds comes out as zeros. `h` and `y` may
+    each be `x` or `residual`."""
     x_at, gamma_at, res_at, h_at = _rms_inputs(x, rows, C, c_valid, eps, gamma, residual, h)
     n = rows * C
     y_at = _operand("y", y, torch.bfloat16, n)

@@ -34,6 +34,7 @@ def _lists():
     yield "each type", [make(n, t) for t in TYPES for n in (1, 7, 8, 9, 4095, 4096, 4097, 100_003)]
     yield "none and empty ones", [make(0, torch.float32), make(5, torch.bfloat16), make(0, torch.float16)]
     yield "many small ones", [make(n % 300 + 1, TYPES[n % 3]) for n in range(1000)]
+    yield "more than one table holds", [make(n % 37 if n % 9 else 0, TYPES[n % 3]) for n in range(4000)]
     yield "one large one", [make(9_999_991, torch.float32)]
     yield "large ones of 16 bits", [make(3_000_001, torch.bfloat16), make(2_000_003, torch.float16)]
     flat = make(50_000, torch.float32)
@@ -43,7 +44,7 @@ def _lists():
     yield "other orders", [make(64 * 48, torch.float32).view(64, 48).t(), make(24 * 12, torch.float32).view(2, 3, 6, 8).permute(0, 3, 1, 2)]
 
 
-@pytest.mark.parametrize("i", range(9))
+@pytest.mark.parametrize("i", range(10))
 @pytest.mark.parametrize("scale,share", [(1.0, 0.37), (0.125, 1.0 + 1e-3), (4.0, 0.9)])
 def test_norm_and_clipping(i, scale, share):
     name, tensors = list(_lists())[i]
@@ -213,10 +214,10 @@ def test_refusals_that_need_a_device():
         K.grad_norm([t], 1.0, torch.zeros(2), ws)
     with pytest.raises(ValueError, match="scratch"):
         K.grad_norm([t], 1.0, out, ws[1:])
-    for bound in (0.0, -1.0, float("nan")):
+    for bound in (0.0, -1.0, float("nan"), 1e-60):
         with pytest.raises(ValueError, match="norm"):
             K.grad_norm([t], bound, out, ws)
-    for scale in (0.0, -1.0, float("nan"), float("inf")):
+    for scale in (0.0, -1.0, float("nan"), float("inf"), 1e-60, 1e39):
         with pytest.raises(ValueError, match="scale"):
             K.grad_norm([t], 1.0, out, ws, scale=scale)
         with pytest.raises(ValueError, match="scale"):

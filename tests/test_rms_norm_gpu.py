@@ -162,6 +162,9 @@ def test_rows_without_anything_and_rows_with_infinities():
     assert (y[1] == 0).all() and torch.equal(y[0], y[5]) and y[0].isfinite().all()
     assert y[2, 3].isnan() and (y[2, :3] == 0).all() and y[3].isnan().all()
     assert (y[4] == 0).all()        # squares of the type's lowest value pass fp32
+    z = torch.empty_like(y)
+    K.rms_norm_fwd(x, rows, C, C, EPS, gamma, z, relu=True)
+    assert z[2, 3].isnan() and z[3].isnan().all() and torch.equal(z[:2], y[:2]) and (z[4] == 0).all()
     q, scales = torch.empty((rows, C), device="cuda", dtype=torch.float8_e4m3fn), torch.empty(rows, device="cuda")
     K.rms_norm_fwd_e4m3(x, rows, C, C, EPS, gamma, q, scales)
     assert scales[1] == 1 and (q[1].float() == 0).all() and (q[0].float() == 448).all()
