@@ -413,8 +413,8 @@ def _stream_of(**tensors):
     """The current stream of the current device, where all of the tensors (or None) have to be."""
     devices = {t.get_device() for t in tensors.values() if t is not None}
     here = devices.pop()
-    if not devices and here >= 0 and here == torch.cuda.current_device():
-        return stream_handle()
+    if not devices and here >= 0 and here == torch._C._cuda_getDevice():
+        return torch._C._cuda_getCurrentRawStream(here)
     for name, t in tensors.items():
         if t is not None and not t.is_cuda:
             raise ValueError(f"{name} has to be on a GPU, not on {t.device}")
