@@ -20,9 +20,9 @@ struct SgdArgs : SgdHyper {
   long long n;
 };
 
-// CLIP: the gradients have just been read for their norm, and part of them is still in the L2: the other streams pass through it
-// as what is not needed again (11.7 M parameters, norm and sweep: 54.4 -> 51.9 us; 62.4 M: 281 -> 277).
-template <bool CLIP>
+// CLIP: the gradients count times clip[1]. They have just been read for their norm, and part of them is still in the L2: with PASS,
+// the other streams go through it as what is not needed again.
+template <bool CLIP, bool PASS>
 __global__ void sgd_fused_kernel(const SgdArgs a) {
   pdl_prolog();
   SgdHyper h = a;
@@ -36,16 +36,16 @@ __global__ void sgd_fused_kernel(const SgdArgs a) {
   const long long n4 = a.n / 4;
   for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < n4;
        i += (long long)gridDim.x * blockDim.x) {
-    float4 w = CLIP ? __ldcs(reinterpret_cast<float4*>(a.w) + i) : reinterpret_cast<float4*>(a.w)[i];
+    float4 w = PASS ? __ldcs(reinterpret_cast<float4*>(a.w) + i) : reinterpret_cast<float4*>(a.w)[i];
     float4 g = reinterpret_cast<float4*>(a.g)[i];
-    float4 v = a.v ? (CLIP ? __ldcs(reinterpret_cast<float4*>(a.v) + i) : reinterpret_cast<float4*>(a.v)[i]) : make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 v = a.v ? (PASS ? __ldcs(reinterpret_cast<float4*>(a.v) + i) : reinterpret_cast<float4*>(a.v)[i]) : make_float4(0.f, 0.f, 0.f, 0.f);
     if (CLIP && drop) g = make_float4(0.f, 0.f, 0.f, 0.f);
     sgd_elem(w.x, g.x, v.x, h);
     sgd_elem(w.y, g.y, v.y, h);
     sgd_elem(w.z, g.z, v.z, h);
     sgd_elem(w.w, g.w, v.w, h);
     auto put = [&](float* to, const float4& x) {
-      if (CLIP) __stcs(reinterpret_cast<float4*>(to) + i, x);
+      if (PASS) __stcs(reinterpret_cast<float4*>(to) + i, x);
       else reinterpret_cast<float4*>(to)[i] = x;
     };
     if (a.phase & 3) put(a.w, w);
@@ -56,7 +56,7 @@ __global__ void sgd_fused_kernel(const SgdArgs a) {
       uint2 o;
       o.x = *reinterpret_cast<uint32_t*>(&lo);
       o.y = *reinterpret_cast<uint32_t*>(&hi);
-      if (CLIP) __stcs(reinterpret_cast<uint2*>(a.w16) + i, o);
+      if (PASS) __stcs(reinterpret_cast<uint2*>(a.w16) + i, o);
       else reinterpret_cast<uint2*>(a.w16)[i] = o;
     }
   }
@@ -108,8 +108,12 @@ int rb_sgd_fused(float* w, float* g, float* v, void* w16, long long n, float lr,
   // within a few MB of one another, where 1184 blocks that step through the whole range spread them over all of it.
   // 62.4 M parameters: 279 -> 244 us (26 bytes each: 6.65 TB/s), 11.7 M: 55 -> 51 us, 1 M: 10 us both.
   const int blocks = (int)std::min(std::max(1ll, (n / 4 + 255) / 256), 1ll << 30);
-  if (clip) launch_streaming(sgd_fused_kernel<true>, blocks, 256, 0, st, a);
-  else launch_streaming(sgd_fused_kernel<false>, blocks, 256, 0, st, a);
+  // Clipped sweeps of four million parameters and more pass through the L2 (norm and sweep, with and without, us: 1.5 M 9.6 and 9.5,
+  // 4.3 M 22.6 and 22.7, 6 M 29.2 and 29.7, 11.7 M 51.7 and 54.4, 62.4 M 277 and 281); what smaller ones write fits there, for the
+  // next forward pass.
+  if (clip && n >= 1ll << 22) launch_streaming(sgd_fused_kernel<true, true>, blocks, 256, 0, st, a);
+  else if (clip) launch_streaming(sgd_fused_kernel<true, false>, blocks, 256, 0, st, a);
+  else launch_streaming(sgd_fused_kernel<false, false>, blocks, 256, 0, st, a);
   return RB_LAUNCH_OK();
 }
 
@@ -124,7 +128,7 @@ int rb_sgd_fused_grid(float* w, float* g, float* v, void* w16, long long n, floa
   a.w = w; a.g = g; a.v = v; a.w16 = (bf16*)w16; a.clip = nullptr; a.n = n;
   const long long need = (n / 4 + threads - 1) / threads;
   if (need < blocks) blocks = need < 1 ? 1 : (int)need;
-  launch_pdl(sgd_fused_kernel<false>, blocks, threads, 0, st, a);
+  launch_pdl(sgd_fused_kernel<false, false>, blocks, threads, 0, st, a);
   return RB_LAUNCH_OK();
 }
 

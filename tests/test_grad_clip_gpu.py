@@ -171,7 +171,7 @@ def test_more_than_two_to_the_31_values():
 
 
 @pytest.mark.parametrize("mode", range(6))
-@pytest.mark.parametrize("n", [1, 1025, 300_000])
+@pytest.mark.parametrize("n", [1, 1025, 300_000, 4_194_311])
 def test_clipped_update(mode, n):
     gen = torch.Generator(device="cuda").manual_seed(n + mode)
     w, g, v = (torch.randn(n, generator=gen, device="cuda") for _ in range(3))
