@@ -284,12 +284,21 @@ struct RmsBackArgs {
   int relu;
 };
 
+// Blocks of the backward kernel that the compiler has to leave room for on an SM (0: as it sees fit). Three vectors: two, which leaves
+// no registers for loads ahead and is faster (40000 x 288: 20.4 us against 19.5, with a delta of h 23.7 against 20.9). Four: one,
+// with all its registers (15000 x 1024: 22.5 against 20.8); two would spill (with a delta of h 25.4 against 36.5).
+template <int L, int V>
+struct RmsBackBlocks {
+  enum { n = !L ? 0 : V == 3 ? 2 : V == 4 ? 1 : 0 };
+};
+
 // A thread has the same channels in all its rows and keeps their part of dgamma in registers; the block's rows are joined at the
 // end and the blocks by rms_dgamma_kernel, both in a fixed order (atomic additions would give other last bits every time).
 template <int L, int V, bool ADD>
-__global__ void __launch_bounds__(RmsBlock<L>::most) rms_norm_back_kernel(const RmsBackArgs a) {
+__global__ void __launch_bounds__(RmsBlock<L>::most, RmsBackBlocks<L, V>::n) rms_norm_back_kernel(const RmsBackArgs a) {
   pdl_prolog();
-  constexpr bool EARLY = L || V * (ADD ? 3 : 2) <= 6;   // registers hold the next rows as well
+  // the next rows' loads are under way where there are registers for them
+  constexpr bool EARLY = L ? V != 3 : V * (ADD ? 3 : 2) <= 6;
   __shared__ float slots[2][16];
   __shared__ __align__(16) float part[L ? V * 2048 : 4];
   const RmsLane<L, V> w(a.gamma, a.C, a.c_valid);
@@ -469,11 +478,13 @@ template <int n>
 using N = std::integral_constant<int, n>;
 
 // Calls go(L, V, threads) for rows of C channels. Up to 1024 channels: as few idle lanes as there can be with at most 4 vectors
-// each, and as many lanes where that is equal. Wider rows: one block with two vectors a thread, more where 512 threads do not hold
-// the row. Twice the threads with one vector each wait longer for one another (8000 x 2048: forward 14.8 us against 12.8, into 8
-// bits 19.0 against 13.5, backward 29.3 against 26.0), half of them with four keep less under way (6000 x 2560: backward 30.8
-// against 22.9).
-template <class F>
+// each, and as many lanes where that is equal. Backward passes and bf16 outputs with a residual (`TWO`) rather leave lanes idle than take
+// three vectors each, whose registers leave one block on an SM (100000 x 96: forward with residual 13.7 us against 14.3, backward
+// 15.3 against 15.8, with a delta of h 17.3 against 18.3; 2000 x 96 backward 3.3 against 3.8; forward alone 9.0 against 8.1). Wider rows: one
+// block with two vectors a thread, more where 512 threads do not hold the row. Twice the threads with one vector each wait longer
+// for one another (8000 x 2048: forward 14.8 us against 12.8, into 8 bits 19.0 against 13.5, backward 29.3 against 26.0), half of
+// them with four keep less under way (6000 x 2560: backward 30.8 against 22.9).
+template <bool TWO, class F>
 static void rms_cover(int C, F go) {
   const int cg = C / 8;
   if (cg > 128) {
@@ -486,10 +497,12 @@ static void rms_cover(int C, F go) {
   int lanes = 0, V = 0;
   for (int l = 32; l >= 4; l >>= 1) {
     const int v = ceil_div(cg, l);
-    if ((v <= 1 || v == 3 || l == 32) && v <= 4 && (!lanes || l * v < lanes * V)) { lanes = l; V = v; }
+    const bool built = v == 1 || l == 32 || (v == 3 && !(TWO && cg <= 32));
+    if (built && v <= 4 && (!lanes || l * v < lanes * V)) { lanes = l; V = v; }
   }
-  if (lanes == 4) V == 1 ? go(N<4>(), N<1>(), 256) : go(N<4>(), N<3>(), 256);
-  else if (lanes == 8) V == 1 ? go(N<8>(), N<1>(), 256) : go(N<8>(), N<3>(), 256);
+  constexpr int THREE = TWO ? 1 : 3;      // what three vectors on four or eight lanes are, where they are not built
+  if (lanes == 4) V == 1 ? go(N<4>(), N<1>(), 256) : go(N<4>(), N<THREE>(), 256);
+  else if (lanes == 8) V == 1 ? go(N<8>(), N<1>(), 256) : go(N<8>(), N<THREE>(), 256);
   else if (lanes == 16) V == 1 ? go(N<16>(), N<1>(), 256) : go(N<16>(), N<3>(), 256);
   else if (V == 1) go(N<32>(), N<1>(), 256);
   else if (V == 2) go(N<32>(), N<2>(), 256);
@@ -507,16 +520,17 @@ int rb_rms_norm_fwd(const void* x, const void* residual, void* h, void* y, void*
   if (rows == 0) return 0;
   const RmsArgs a{(const bf16*)x, (const bf16*)residual, (bf16*)h, (bf16*)y, (uint8_t*)q, scales, rstd, gamma, rows, C, c_valid,
                   eps, 1.f / (float)c_valid, relu};
-  rms_cover(C, [&](auto lanes, auto vectors, int threads) {
-    constexpr int L = decltype(lanes)::value, V = decltype(vectors)::value;
-    auto go = [&](auto res, auto q8) {
-      constexpr auto kern = rms_norm_kernel<L, V, decltype(res)::value, decltype(q8)::value>;
+  auto run = [&](auto res, auto q8) {
+    constexpr bool RES = decltype(res)::value, Q8 = decltype(q8)::value;
+    rms_cover<RES && !Q8>(C, [&](auto lanes, auto vectors, int threads) {
+      constexpr int L = decltype(lanes)::value;
+      constexpr auto kern = rms_norm_kernel<L, decltype(vectors)::value, RES, Q8>;
       const long long need = (rows + RmsBlock<L>::rows - 1) / RmsBlock<L>::rows, most = 148ll * blocks_per_sm<kern>(threads);
       launch_pdl(kern, (unsigned)std::min(need, most), threads, 0, st, a);
-    };
-    if (residual) q ? go(std::true_type(), std::true_type()) : go(std::true_type(), std::false_type());
-    else q ? go(std::false_type(), std::true_type()) : go(std::false_type(), std::false_type());
-  });
+    });
+  };
+  if (residual) q ? run(std::true_type(), std::true_type()) : run(std::true_type(), std::false_type());
+  else q ? run(std::false_type(), std::true_type()) : run(std::false_type(), std::false_type());
   return RB_LAUNCH_OK();
 }
 
@@ -528,7 +542,7 @@ int rb_rms_norm_bwd(const void* h, const void* dy, const void* add, void* dx, co
   const RmsBackArgs a{(const bf16*)h, (const bf16*)dy, (const bf16*)add, (bf16*)dx, rstd, gamma, dgamma, ws, rows, C, c_valid,
                       1.f / (float)c_valid, relu};
   int blocks = 0;
-  rms_cover(C, [&](auto lanes, auto vectors, int threads) {
+  rms_cover<true>(C, [&](auto lanes, auto vectors, int threads) {
     constexpr int L = decltype(lanes)::value, V = decltype(vectors)::value;
     auto go = [&](auto with) {
       constexpr auto kern = rms_norm_back_kernel<L, V, decltype(with)::value>;
