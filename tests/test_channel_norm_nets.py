@@ -71,9 +71,8 @@ def _sweep(w, g, v, w16, n, lr, mu, l2, grad_scale, mode, phase=7, clip=None):
 
 
 def _install(monkeypatch):
-    scratch = K.rms_norm_scratch
     kernel_emulation.install(monkeypatch)
-    for name, fn in {"rms_norm_fwd": _fwd, "rms_norm_bwd": _bwd, "rms_norm_scratch": scratch, "grad_norm": _norm,
+    for name, fn in {"rms_norm_fwd": _fwd, "rms_norm_bwd": _bwd, "rms_norm_scratch": lambda C_, device: torch.zeros(K.RMS_SCRATCH_ROWS * C_), "grad_norm": _norm,
                      "grad_list": list, "grad_norm_scratch": lambda device: None, "sgd_fused": _sweep}.items():
         monkeypatch.setattr(K, name, fn)
 
