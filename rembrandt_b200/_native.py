@@ -80,8 +80,8 @@ _CUDA_SIGS = {
     "rb_axpy_shadow": [vp, vp, vp, i64, f32, vp],
     "rb_axpby": [vp, vp, i64, f32, f32, vp],
     # grad_clip.cu
-    "rb_grad_norm": [vp, vp, vp, i32, f32, f32, vp, vp, vp],
-    "rb_clip_grads": [vp, vp, vp, i32, f32, vp, vp],
+    "rb_grad_norm": [vp, f32, f32, vp, vp, vp],
+    "rb_clip_grads": [vp, f32, vp, vp],
     # input_pipeline.cu
     "rb_input_u8": [vp, vp, vp] + [i32] * 20 + [f32, f32, f32, vp, vp, u64, u32, vp, vp],
     "rb_var_input_u8": [vp, vp, vp, vp, i64] + [i32] * 14 + [f32, vp, f32, vp, vp, u64, u32, vp, vp],
@@ -95,8 +95,8 @@ _CUDA_SIGS = {
     "rb_bn_fold": [vp, vp, i32, vp, vp],
     "rb_bn_bwd": [vp, vp, vp, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp],
     # rms_norm.cu
-    "rb_rms_norm_fwd": [vp, vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, f32, i32, vp],
-    "rb_rms_norm_bwd": [vp, vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, vp],
+    "rb_rms_norm_fwd": [vp, vp],
+    "rb_rms_norm_bwd": [vp, vp],
 }
 
 

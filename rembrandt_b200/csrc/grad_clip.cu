@@ -16,6 +16,7 @@
 #include <cuda_fp16.h>
 #include <algorithm>
 #include <utility>
+#include <string.h>
 
 namespace rb {
 
@@ -311,8 +312,23 @@ static bool fill_tables(const void* const* at, const long long* n, const int* ty
   }
   return true;
 }
+// A list of gradients as calls hand it over: host arrays of addresses, numbers of values and types (0 fp32, 1 bf16, 2 fp16).
+struct GradListRecord {
+  const void* const* at;
+  const long long* n;
+  const int* types;
+  long long count;
+};
+static_assert(sizeof(GradListRecord) == 32, "as ops/native_ops.py packs it");
+
 template <class F>
-static bool for_tables(const void* const* at, const long long* n, const int* types, int count, F f) {
+static bool for_tables(const void* list, F f) {
+  GradListRecord r;
+  memcpy(&r, list, sizeof(r));
+  const void* const* at = r.at;
+  const long long* n = r.n;
+  const int* types = r.types;
+  const int count = r.count < 0 || r.count > 1 << 30 ? -1 : (int)r.count;
   if (count < 0 || (count && (!at || !n || !types))) return false;
   for (int i = 0; i < count; ++i) {
     if (types[i] < 0 || types[i] > 2 || n[i] < 0 || n[i] > (1ll << 40)) return false;
@@ -323,14 +339,13 @@ static bool for_tables(const void* const* at, const long long* n, const int* typ
 
 extern "C" {
 
-// at, n, types: host arrays of `count` addresses, numbers of values and types (0 fp32, 1 bf16, 2 fp16). ws: 740 doubles.
-int rb_grad_norm(const void* const* at, const long long* n, const int* types, int count, float scale, float max_norm,
-                 float* out, double* ws, cudaStream_t st) {
-  if (!out || !ws || !(max_norm > 0.f)) return -10;
+// list: a packed GradListRecord; ws: 740 doubles.
+int rb_grad_norm(const void* list, float scale, float max_norm, float* out, double* ws, cudaStream_t st) {
+  if (!list || !out || !ws || !(max_norm > 0.f)) return -10;
   int again = 0;
   bool done = false;
-  const bool ok = for_tables(at, n, types, count, [&](const auto& t) {
-    done = !again && t.chunks <= SMALL_CHUNKS && count <= FEW;
+  const bool ok = for_tables(list, [&](const auto& t) {
+    done = !again && t.chunks <= SMALL_CHUNKS && sizeof(t.first) / 4 == FEW;
     if (done) {
       launch_pdl(grad_norm_small_kernel<sizeof(t.first) / 4>, CLUSTER, 1024, 0, st, t, out, (double)scale, max_norm);
       return;
@@ -345,10 +360,9 @@ int rb_grad_norm(const void* const* at, const long long* n, const int* types, in
   return RB_LAUNCH_OK();
 }
 
-int rb_clip_grads(const void* const* at, const long long* n, const int* types, int count, float scale, const float* out,
-                  cudaStream_t st) {
-  if (!out) return -10;
-  const bool ok = for_tables(at, n, types, count, [&](const auto& t) {
+int rb_clip_grads(const void* list, float scale, const float* out, cudaStream_t st) {
+  if (!list || !out) return -10;
+  const bool ok = for_tables(list, [&](const auto& t) {
     const int run = ceil_div(t.chunks, CLIP_BLOCKS);
     launch_pdl(clip_kernel<sizeof(t.first) / 4>, ceil_div(t.chunks, run), 256, 0, st, t, out, scale, run);
   });

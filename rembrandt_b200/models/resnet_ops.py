@@ -237,7 +237,7 @@ def check_rms_norm(cp, eps):
     """Refuses what the kernels of the normalisation over channels would refuse when they are first called."""
     if cp > K.RMS_MAX_CHANNELS:
         raise ValueError(f"a normalisation over channels takes at most {K.RMS_MAX_CHANNELS} channels, not {cp}")
-    if not 2.0 ** -126 <= eps < float("inf"):
+    if not 2.0 ** -126 <= eps < 2.0 ** 127:
         raise ValueError(f"the epsilon of a normalisation has to be a positive float32, not {eps}")
 
 

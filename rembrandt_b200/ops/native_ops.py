@@ -12,6 +12,8 @@ The functions raise ``NativeError`` if a launcher reports a problem; there is no
 """
 from __future__ import annotations
 
+import struct
+
 import torch
 
 from .. import _native
@@ -465,7 +467,8 @@ class GradList:
         self._at = (C_.c_void_p * n)(*(t.data_ptr() for t in self.tensors))
         self._n = (C_.c_longlong * n)(*(t.numel() for t in self.tensors))
         self._types = (C_.c_int * n)(*(_GRAD_TYPES[t.dtype] for t in self.tensors))
-        self.args = (C_.addressof(self._at), C_.addressof(self._n), C_.addressof(self._types), n)
+        # `GradListRecord` (csrc/grad_clip.cu)
+        self.record = struct.pack("<3Qq", C_.addressof(self._at), C_.addressof(self._n), C_.addressof(self._types), n)
 
 
 def _check_same_device(tensors):
@@ -498,7 +501,7 @@ def grad_norm(tensors, max_norm, out, ws, scale=1.0):
     out_at = _operand("out", out, torch.float32, 2, 4)
     ws_at = _operand("scratch", ws, torch.float64, GRAD_NORM_SUMS)
     stream = _stream_of(out=out, scratch=ws, gradient=tensors.first)
-    check(_native.cuda().rb_grad_norm(*tensors.args, scale, max_norm, out_at, ws_at, stream), "rb_grad_norm")
+    check(_native.cuda().rb_grad_norm(tensors.record, scale, max_norm, out_at, ws_at, stream), "rb_grad_norm")
 
 
 def _check_scale(scale):
@@ -513,7 +516,7 @@ def clip_grads(tensors, out, scale=1.0):
     _check_scale(scale)
     out_at = _operand("out", out, torch.float32, 2, 4)
     stream = _stream_of(out=out, gradient=tensors.first)
-    check(_native.cuda().rb_clip_grads(*tensors.args, scale, out_at, stream), "rb_clip_grads")
+    check(_native.cuda().rb_clip_grads(tensors.record, scale, out_at, stream), "rb_clip_grads")
 
 
 def axpy_shadow(w, v, w16, n, s):
@@ -629,6 +632,9 @@ def bn_bwd_ws(x, dy, y_relu, rows, C, c_valid, ws, mean, istd, gamma, dgamma, db
 
 # ------------------------------------------------------------------ normalisation over channels
 RMS_MAX_CHANNELS = 16384
+# `RmsFwdCall` and `RmsBwdCall` (csrc/rms_norm.cu)
+_RMS_FWD_CALL = struct.Struct("<8Qq2ifi")
+_RMS_BWD_CALL = struct.Struct("<8Qq4i")
 
 
 def _check_rms_shape(rows, C, c_valid):
@@ -638,7 +644,7 @@ def _check_rms_shape(rows, C, c_valid):
 
 
 def _check_rms_eps(eps):
-    if not 2.0 ** -126 <= eps < float("inf"):
+    if not 2.0 ** -126 <= eps < 2.0 ** 127:
         raise ValueError(f"an epsilon has to be a positive float32, not {eps}")
 
 
@@ -655,7 +661,7 @@ def _rms_inputs(x, rows, C, c_valid, eps, gamma, residual, h):
     n = rows * C
     x_at = _operand("x", x, torch.bfloat16, n)
     gamma_at = _operand("gamma", gamma, torch.float32, C)
-    res_at = h_at = None
+    res_at = h_at = 0
     if residual is not None:
         res_at = _operand("residual", residual, torch.bfloat16, n)
     if h is not None:
@@ -677,14 +683,14 @@ def rms_norm_fwd(x, rows, C, c_valid, eps, gamma, y, rstd=None, residual=None, h
     n = rows * C
     y_at = _operand("y", y, torch.bfloat16, n)
     _check_apart("y", y_at, 2 * n, "x", x_at, 2 * n, True)
-    if res_at is not None:
+    if res_at:
         _check_apart("y", y_at, 2 * n, "residual", res_at, 2 * n, True)
-    if h_at is not None:
+    if h_at:
         _check_apart("y", y_at, 2 * n, "h", h_at, 2 * n, False)
-    rstd_at = None if rstd is None else _operand("rstd", rstd, torch.float32, rows, 4)
+    rstd_at = 0 if rstd is None else _operand("rstd", rstd, torch.float32, rows, 4)
     stream = _stream_of(x=x, gamma=gamma, y=y, residual=residual, h=h, rstd=rstd)
-    check(_native.cuda().rb_rms_norm_fwd(x_at, res_at, h_at, y_at, None, None, rstd_at, gamma_at, rows, C, c_valid, eps,
-                                         1 if relu else 0, stream), "rb_rms_norm_fwd")
+    call = _RMS_FWD_CALL.pack(x_at, res_at, h_at, y_at, 0, 0, rstd_at, gamma_at, rows, C, c_valid, eps, 1 if relu else 0)
+    check(_native.cuda().rb_rms_norm_fwd(call, stream), "rb_rms_norm_fwd")
 
 
 def rms_norm_fwd_e4m3(x, rows, C, c_valid, eps, gamma, q, scales, residual=None, h=None, relu=False):
@@ -696,11 +702,11 @@ def rms_norm_fwd_e4m3(x, rows, C, c_valid, eps, gamma, q, scales, residual=None,
     q_at = _operand("q", q, torch.float8_e4m3fn, n)
     scales_at = _operand("scales", scales, torch.float32, rows, 4)
     for other, at in (("x", x_at), ("residual", res_at), ("h", h_at)):
-        if at is not None:
+        if at:
             _check_apart("q", q_at, n, other, at, 2 * n, False)
     stream = _stream_of(x=x, gamma=gamma, q=q, scales=scales, residual=residual, h=h)
-    check(_native.cuda().rb_rms_norm_fwd(x_at, res_at, h_at, None, q_at, scales_at, None, gamma_at, rows, C, c_valid, eps,
-                                         1 if relu else 0, stream), "rb_rms_norm_fwd")
+    call = _RMS_FWD_CALL.pack(x_at, res_at, h_at, 0, q_at, scales_at, 0, gamma_at, rows, C, c_valid, eps, 1 if relu else 0)
+    check(_native.cuda().rb_rms_norm_fwd(call, stream), "rb_rms_norm_fwd")
 
 
 RMS_SCRATCH_ROWS = 592      # most blocks whose sums a backward pass joins; twice as many for 1032 to 2048 channels
@@ -727,14 +733,14 @@ def rms_norm_bwd(h, dy, rows, C, c_valid, rstd, gamma, dgamma, dx, ws, add=None,
     h_at = _operand("h", h, torch.bfloat16, n)
     dy_at = _operand("dy", dy, torch.bfloat16, n)
     dx_at = _operand("dx", dx, torch.bfloat16, n)
-    add_at = None if add is None else _operand("add", add, torch.bfloat16, n)
+    add_at = 0 if add is None else _operand("add", add, torch.bfloat16, n)
     for other, at in (("h", h_at), ("dy", dy_at), ("add", add_at)):
-        if at is not None:
+        if at:
             _check_apart("dx", dx_at, 2 * n, other, at, 2 * n, True)
     rstd_at = _operand("rstd", rstd, torch.float32, rows, 4)
     gamma_at = _operand("gamma", gamma, torch.float32, C)
     dgamma_at = _operand("dgamma", dgamma, torch.float32, C)
     ws_at = _operand("scratch", ws, torch.float32, _rms_scratch_rows(C) * C)
     stream = _stream_of(h=h, dy=dy, dx=dx, rstd=rstd, gamma=gamma, dgamma=dgamma, scratch=ws, add=add)
-    check(_native.cuda().rb_rms_norm_bwd(h_at, dy_at, add_at, dx_at, rstd_at, gamma_at, dgamma_at, ws_at, rows, C, c_valid,
-                                         1 if relu else 0, stream), "rb_rms_norm_bwd")
+    call = _RMS_BWD_CALL.pack(h_at, dy_at, add_at, dx_at, rstd_at, gamma_at, dgamma_at, ws_at, rows, C, c_valid, 1 if relu else 0, 0)
+    check(_native.cuda().rb_rms_norm_bwd(call, stream), "rb_rms_norm_bwd")

@@ -61,7 +61,7 @@ def test_shapes(call):
 
 
 @pytest.mark.parametrize("call", [_fwd, _fwd8])
-@pytest.mark.parametrize("eps", [0.0, -1e-5, float("nan"), float("inf"), 1e-40])
+@pytest.mark.parametrize("eps", [0.0, -1e-5, float("nan"), float("inf"), 1e-40, 1e39])
 def test_epsilons(call, eps):
     with pytest.raises(ValueError, match="epsilon"):
         call(_good() | {"eps": eps})

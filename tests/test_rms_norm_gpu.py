@@ -237,6 +237,11 @@ def test_no_rows():
     K.rms_norm_fwd_e4m3(x, 0, 64, 64, EPS, gamma, q, rstd)
     K.rms_norm_bwd(x, x, 0, 64, 64, rstd, gamma, dgamma, y, K.rms_norm_scratch(64, "cuda"))
     assert (y == 5).all() and rstd[0] == 5 and (dgamma == 3).all() and (q.float() == 1).all()
+    none, no_rows = x[:0].clone(), rstd[:0].clone()
+    K.rms_norm_fwd(none, 0, 64, 64, EPS, gamma, none.clone(), rstd=no_rows, residual=none.clone(), h=none.clone())
+    K.rms_norm_fwd_e4m3(none, 0, 64, 64, EPS, gamma, none.to(torch.float8_e4m3fn), no_rows, residual=none.clone(), h=none.clone())
+    K.rms_norm_bwd(none, none, 0, 64, 64, no_rows, gamma, dgamma, none.clone(), K.rms_norm_scratch(64, "cuda"), add=none)
+    assert (dgamma == 3).all()
 
 
 def test_two_graphs_with_their_own_scratch_run_at_the_same_time():
