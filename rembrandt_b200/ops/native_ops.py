@@ -12,6 +12,7 @@ The functions raise ``NativeError`` if a launcher reports a problem; there is no
 """
 from __future__ import annotations
 
+import array
 import struct
 
 import torch
@@ -429,8 +430,6 @@ GRAD_NORM_SUMS = 740       # 64-bit sums that `grad_norm` keeps between its laun
 
 def _is_dense(t):
     """Whether the values of `t` fill one range of memory, in any order of its dimensions."""
-    if t.is_contiguous():
-        return True
     step = 1
     for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda p: p[1]):
         if stride != step:
@@ -446,37 +445,36 @@ class GradList:
     gradients are new tensors in every step gives `grad_norm` and `clip_grads` the tensors themselves."""
 
     def __init__(self, tensors):
-        import ctypes as C_
-        self.tensors = tuple(tensors)
-        ends = []
-        for i, t in enumerate(self.tensors):
-            if not torch.is_tensor(t) or t.layout != torch.strided or t.dtype not in _GRAD_TYPES:
+        self.tensors = tensors = tuple(tensors)
+        at, sizes, types, ends, devices = array.array("Q"), array.array("q"), array.array("i"), [], set()
+        for i, t in enumerate(tensors):
+            kind = _GRAD_TYPES.get(t.dtype) if isinstance(t, torch.Tensor) else None
+            if kind is None or t.layout is not torch.strided:
                 raise ValueError(f"gradient {i} has to be a float32, bfloat16 or float16 tensor, not "
-                                 f"{t.dtype if torch.is_tensor(t) else type(t).__name__}")
-            if not _is_dense(t):
+                                 f"{t.dtype if isinstance(t, torch.Tensor) else type(t).__name__}")
+            if not (t.is_contiguous() or _is_dense(t)):
                 raise ValueError(f"gradient {i} {tuple(t.shape)} with strides {t.stride()} leaves gaps in memory")
-            if t.numel():
-                ends.append((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), i))
+            address, n = t.data_ptr(), t.numel()
+            at.append(address)
+            sizes.append(n)
+            types.append(kind)
+            devices.add(t.get_device())
+            if n:
+                ends.append((address, address + n * (4 if kind == 0 else 2), i))
         ends.sort()
-        for (_, end, i), (at, _, j) in zip(ends, ends[1:]):
-            if at < end:
+        for (_, end, i), (start, _, j) in zip(ends, ends[1:]):
+            if start < end:
                 raise ValueError(f"gradients {i} and {j} overlap")
-        _check_same_device(self.tensors)
-        n = self.count = len(self.tensors)
-        self.first = self.tensors[0] if n else None
-        self._at = (C_.c_void_p * n)(*(t.data_ptr() for t in self.tensors))
-        self._n = (C_.c_longlong * n)(*(t.numel() for t in self.tensors))
-        self._types = (C_.c_int * n)(*(_GRAD_TYPES[t.dtype] for t in self.tensors))
-        # `GradListRecord` (csrc/grad_clip.cu)
-        self.record = struct.pack("<3Qq", C_.addressof(self._at), C_.addressof(self._n), C_.addressof(self._types), n)
-
-
-def _check_same_device(tensors):
-    for i, t in enumerate(tensors):
-        if not t.is_cuda:
-            raise ValueError(f"gradient {i} has to be on a GPU, not on {t.device}")
-        if t.device != tensors[0].device:
-            raise ValueError(f"gradient {i} is on {t.device}, the first on {tensors[0].device}")
+        if len(devices) > 1 or -1 in devices:
+            for i, t in enumerate(tensors):
+                if not t.is_cuda:
+                    raise ValueError(f"gradient {i} has to be on a GPU, not on {t.device}")
+                if t.device != tensors[0].device:
+                    raise ValueError(f"gradient {i} is on {t.device}, the first on {tensors[0].device}")
+        self.first = tensors[0] if tensors else None
+        # `GradListRecord` (csrc/grad_clip.cu), and the arrays that it points to
+        self._arrays = at, sizes, types
+        self.record = struct.pack("<3Qq", *(a.buffer_info()[0] for a in self._arrays), len(tensors))
 
 
 def grad_list(tensors):
