@@ -31,17 +31,17 @@ class SgdStepper:
         self.clip = torch.zeros(2, dtype=torch.float32, device=net.device) if net.is_cuda and self.clip_norm else None
         self._clip_host = (0.0, 1.0)
         self._clip_ws = K.grad_norm_scratch(net.device) if self.clip is not None else None
-        self._clip_list = None
+        self._clip_list = self._clip_of = None
 
     def _measure(self, grad_scale):
         """Norm and coefficient of all gradients, as they are now."""
         net = self.net
         if net.is_cuda:
-            if self._clip_list is None:
-                self._clip_list = K.grad_list([net.grads])
+            if self._clip_of is not net.grads:
+                self._clip_list, self._clip_of = K.grad_list([net.grads]), net.grads
             K.grad_norm(self._clip_list, self.clip_norm, self.clip, self._clip_ws, scale=grad_scale)
         else:
-            norm = abs(grad_scale) * float(torch.linalg.vector_norm(net.grads.detach(), dtype=torch.float64))
+            norm = float((grad_scale * torch.linalg.vector_norm(net.grads.detach(), dtype=torch.float64)).float())
             self._clip_host = (norm, clip_coefficient(norm, self.clip_norm))
 
     def grad_norm(self):
@@ -68,8 +68,9 @@ class SgdStepper:
         hi = net.flat_len if hi is None else hi
         clip = {}
         if self.clip_norm:
-            if (lo, hi) != (0, net.flat_len):
-                raise ValueError("gradients are clipped by the norm of all of them: the sweep cannot take a part")
+            if (lo, hi) != (0, net.flat_len) or grid is not None:
+                raise ValueError("gradients are clipped by the norm of all of them: the sweep can neither take a part nor run beside "
+                                 "backward")
             if phase & 1:        # a later phase of the iteration goes by the norm that this one has found
                 self._measure(grad_scale)
             if net.is_cuda:

@@ -332,8 +332,9 @@ def test_what_cannot_be_clipped_is_refused():
         with pytest.raises(ValueError, match="norm"):
             SgdStepper(net, Momentum.UPDATE, 0.9, 0.0, clip_norm=bad)
     st = SgdStepper(net, Momentum.UPDATE, 0.9, 0.0, clip_norm=1.0)
-    with pytest.raises(ValueError, match="part"):
-        st.step(0.1, lo=0, hi=64)
+    for part in ({"lo": 0, "hi": 64}, {"lo": 64}, {"grid": (296, 128)}):
+        with pytest.raises(ValueError, match="part"):
+            st.step(0.1, **part)
     assert SgdStepper(net, Momentum.UPDATE, 0.9, 0.0).grad_norm() is None
     opt = SgdOptConfig(minibatch_size=4, clip_norm=1.0)
     with pytest.raises(ValueError, match="clip_norm"):
