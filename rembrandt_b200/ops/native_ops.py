@@ -388,12 +388,15 @@ def rate_args(lr):
 
 
 def sgd_fused(w, g, v, w16, n, lr, mu, l2, grad_scale, mode, phase=7, clip=None):
-    """`clip`: what `grad_norm` has written (float32 [2]); the gradients count times its coefficient, and as zeros where that
-    is 0."""
-    if clip is not None:
+    """`clip`: what `grad_norm` has written (float32 [2]), on the device of the others, which is the current one; the gradients
+    count times its coefficient, and as zeros where that is 0."""
+    if clip is None:
+        stream = stream_handle()
+    else:
         _operand("clip", clip, torch.float32, 2, align=4)
+        stream = _stream_of(clip=clip, w=w, g=g, v=v, w16=w16)
     check(_native.cuda().rb_sgd_fused(ptr(w), ptr(g), ptr(v), ptr(w16), n, *rate_args(lr), mu, l2, grad_scale, mode, phase,
-                                      ptr(clip), stream_handle()), "rb_sgd_fused")
+                                      ptr(clip), stream), "rb_sgd_fused")
 
 
 def sgd_fused_grid(w, g, v, w16, n, lr, mu, l2, grad_scale, mode, phase=7, blocks=296, threads=128):
