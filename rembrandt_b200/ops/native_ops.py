@@ -13,6 +13,7 @@ The functions raise ``NativeError`` if a launcher reports a problem; there is no
 from __future__ import annotations
 
 import array
+import bisect
 import struct
 
 import torch
@@ -390,13 +391,17 @@ def rate_args(lr):
 def sgd_fused(w, g, v, w16, n, lr, mu, l2, grad_scale, mode, phase=7, clip=None):
     """`clip`: what `grad_norm` has written (float32 [2]), on the device of the others, which is the current one; the gradients
     count times its coefficient, and as zeros where that is 0."""
+    w_at, g_at, v_at, w16_at = ptr(w), ptr(g), ptr(v), ptr(w16)
     if clip is None:
-        stream = stream_handle()
+        clip_at, stream = None, stream_handle()
     else:
-        _operand("clip", clip, torch.float32, 2, align=4)
-        stream = _stream_of(clip=clip, w=w, g=g, v=v, w16=w16)
-    check(_native.cuda().rb_sgd_fused(ptr(w), ptr(g), ptr(v), ptr(w16), n, *rate_args(lr), mu, l2, grad_scale, mode, phase,
-                                      ptr(clip), stream), "rb_sgd_fused")
+        clip_at = _operand("clip", clip, torch.float32, 2, 4)
+        end, reach = clip_at + 8, clip_at - 4 * n
+        if (reach < w_at < end or reach < g_at < end or v_at and reach < v_at < end or w16_at and clip_at - 2 * n < w16_at < end):
+            raise ValueError("clip overlaps what the sweep writes")
+        stream = _stream_of("clip w g v w16", clip, w, g, v, w16)
+    check(_native.cuda().rb_sgd_fused(w_at, g_at, v_at, w16_at, n, *rate_args(lr), mu, l2, grad_scale, mode, phase, clip_at,
+                                      stream), "rb_sgd_fused")
 
 
 def sgd_fused_grid(w, g, v, w16, n, lr, mu, l2, grad_scale, mode, phase=7, blocks=296, threads=128):
@@ -415,16 +420,20 @@ def _operand(name, t, dtype, n, align=16):
     raise ValueError(f"{name} has to be {n} contiguous values of {dtype} on a {align}-byte boundary, not {what}")
 
 
-def _stream_of(**tensors):
-    """The current stream of the current device, where all of the tensors (or None) have to be."""
-    devices = {t.get_device() for t in tensors.values() if t is not None}
-    here = devices.pop()
-    if not devices and here >= 0 and here == torch._C._cuda_getDevice():
-        return torch._C._cuda_getCurrentRawStream(here)
-    for name, t in tensors.items():
-        if t is not None and not t.is_cuda:
+def _stream_of(names, *tensors):
+    """The current stream of the current device, where all of the tensors (or None) have to be; the first is not None."""
+    here = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            break
+    else:
+        if here >= 0 and here == torch._C._cuda_getDevice():
+            return torch._C._cuda_getCurrentRawStream(here)
+    given = [(name, t) for name, t in zip(names.split(), tensors) if t is not None]
+    for name, t in given:
+        if not t.is_cuda:
             raise ValueError(f"{name} has to be on a GPU, not on {t.device}")
-    raise ValueError("not all on the current device: " + ", ".join(f"{n} on {t.device}" for n, t in tensors.items() if t is not None))
+    raise ValueError("not all on the current device: " + ", ".join(f"{n} on {t.device}" for n, t in given))
 
 
 _GRAD_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -475,9 +484,17 @@ class GradList:
                 if t.device != tensors[0].device:
                     raise ValueError(f"gradient {i} is on {t.device}, the first on {tensors[0].device}")
         self.first = tensors[0] if tensors else None
+        self._starts, self._ends = [e[0] for e in ends], [e[1] for e in ends]
+        self.start, self.end = (ends[0][0], ends[-1][1]) if ends else (0, 0)     # of all of them
         # `GradListRecord` (csrc/grad_clip.cu), and the arrays that it points to
         self._arrays = at, sizes, types
         self.record = struct.pack("<3Qq", *(a.buffer_info()[0] for a in self._arrays), len(tensors))
+
+    def check_apart(self, name, at, size):
+        """ValueError where a gradient has any of the `size` bytes at `at`."""
+        i = bisect.bisect_left(self._starts, at + size) - 1      # the last one that starts before their end
+        if i >= 0 and self._ends[i] > at:
+            raise ValueError(f"{name} overlaps a gradient")
 
 
 def grad_list(tensors):
@@ -493,15 +510,21 @@ def grad_norm_scratch(device):
 def grad_norm(tensors, max_norm, out, ws, scale=1.0):
     """out[0] = scale * (sum of the squares of all values of `tensors`)^1/2, their global norm; out[1] = the coefficient that
     brings it down to `max_norm`: max_norm / out[0] where the norm is larger, 1 where it is not, 0 where it is no finite
-    float32. `out`: float32 [2]; `tensors`: a `GradList` or tensors that make one; `ws`: `grad_norm_scratch`. The sum is
-    taken in 64 bits and in the same order every time."""
+    float32. `out`: float32 [2]; `tensors`: a `GradList` or tensors that make one; `ws`: `grad_norm_scratch`; none of them
+    overlap. The sum is taken in 64 bits and in the same order every time."""
     tensors, max_norm, scale = grad_list(tensors), float(max_norm), float(scale)
     if not max_norm >= 2.0 ** -149:
         raise ValueError(f"a largest norm has to be a float32 above 0, not {max_norm}")
     _check_scale(scale)
     out_at = _operand("out", out, torch.float32, 2, 4)
     ws_at = _operand("scratch", ws, torch.float64, GRAD_NORM_SUMS)
-    stream = _stream_of(out=out, scratch=ws, gradient=tensors.first)
+    if ws_at - 8 < out_at < ws_at + 8 * GRAD_NORM_SUMS:
+        raise ValueError("out overlaps scratch")
+    if tensors.start < out_at + 8 and out_at < tensors.end:
+        tensors.check_apart("out", out_at, 8)
+    if tensors.start < ws_at + 8 * GRAD_NORM_SUMS and ws_at < tensors.end:
+        tensors.check_apart("scratch", ws_at, 8 * GRAD_NORM_SUMS)
+    stream = _stream_of("out scratch gradient", out, ws, tensors.first)
     check(_native.cuda().rb_grad_norm(tensors.record, scale, max_norm, out_at, ws_at, stream), "rb_grad_norm")
 
 
@@ -516,7 +539,9 @@ def clip_grads(tensors, out, scale=1.0):
     tensors, scale = grad_list(tensors), float(scale)
     _check_scale(scale)
     out_at = _operand("out", out, torch.float32, 2, 4)
-    stream = _stream_of(out=out, gradient=tensors.first)
+    if tensors.start < out_at + 8 and out_at < tensors.end:
+        tensors.check_apart("out", out_at, 8)
+    stream = _stream_of("out gradient", out, tensors.first)
     check(_native.cuda().rb_clip_grads(tensors.record, scale, out_at, stream), "rb_clip_grads")
 
 
@@ -649,10 +674,13 @@ def _check_rms_eps(eps):
         raise ValueError(f"an epsilon has to be a positive float32, not {eps}")
 
 
-def _check_apart(name, at, size, other, other_at, other_size, same):
-    """The `size` bytes at `at` overlap none of another operand's, but may be those where `same`."""
-    if at < other_at + other_size and other_at < at + size and not (same and at == other_at):
-        raise ValueError(f"{name} overlaps {other}")
+def _check_apart(written, *spans):
+    """`spans`: (address, bytes, name) of the operands of a call that overlap, as far as a quick look can tell; those that it
+    writes are the first `written` ones. An input that one of these exactly stands in the place of is not among them."""
+    for i, (at, size, name) in enumerate(spans[:written]):
+        for other_at, other_size, other in spans[i + 1:]:
+            if max(at, other_at) < min(at + size, other_at + other_size):
+                raise ValueError(f"{name} overlaps {other}")
 
 
 def _rms_inputs(x, rows, C, c_valid, eps, gamma, residual, h):
@@ -669,8 +697,6 @@ def _rms_inputs(x, rows, C, c_valid, eps, gamma, residual, h):
         if residual is None:
             raise ValueError("h is x where there is no residual: it is not written")
         h_at = _operand("h", h, torch.bfloat16, n)
-        _check_apart("h", h_at, 2 * n, "x", x_at, 2 * n, True)
-        _check_apart("h", h_at, 2 * n, "residual", res_at, 2 * n, True)
     return x_at, gamma_at, res_at, h_at
 
 
@@ -679,17 +705,22 @@ def rms_norm_fwd(x, rows, C, c_valid, eps, gamma, y, rstd=None, residual=None, h
     row of [rows][C] by its own root mean square. `rstd` [rows] (float32, for `rms_norm_bwd`): the factor that stands for the
     root; `h`: the sum, rounded to bf16 before it is normalised, whether it is stored or not. Channels from `c_valid` on count
     as zeros and are written as such. A row whose squares add up to more than float32 holds comes out as zeros. `h` and `y` may
-    each be `x` or `residual`."""
+    each be `x` or `residual`; nothing else that is written may overlap an operand."""
     x_at, gamma_at, res_at, h_at = _rms_inputs(x, rows, C, c_valid, eps, gamma, residual, h)
     n = rows * C
     y_at = _operand("y", y, torch.bfloat16, n)
-    _check_apart("y", y_at, 2 * n, "x", x_at, 2 * n, True)
-    if res_at:
-        _check_apart("y", y_at, 2 * n, "residual", res_at, 2 * n, True)
-    if h_at:
-        _check_apart("y", y_at, 2 * n, "h", h_at, 2 * n, False)
     rstd_at = 0 if rstd is None else _operand("rstd", rstd, torch.float32, rows, 4)
-    stream = _stream_of(x=x, gamma=gamma, y=y, residual=residual, h=h, rstd=rstd)
+    # y, h and rstd overlap nothing, except for y or h exactly in the place of x or residual
+    x_end, y_end, g_end, r_end, res_end, h_end = x_at + 2 * n, y_at + 2 * n, gamma_at + 4 * C, rstd_at + 4 * rows, res_at + 2 * n, h_at + 2 * n
+    if (y_at < x_end and x_at < y_end and x_at != y_at or y_at < g_end and gamma_at < y_end or
+            rstd_at and (rstd_at < x_end and x_at < r_end or rstd_at < y_end and y_at < r_end or rstd_at < g_end and gamma_at < r_end) or
+            res_at and (y_at < res_end and res_at < y_end and res_at != y_at or rstd_at and rstd_at < res_end and res_at < r_end) or
+            h_at and (h_at < x_end and x_at < h_end and x_at != h_at or h_at < res_end and res_at < h_end and res_at != h_at or
+                      h_at < y_end and y_at < h_end or h_at < g_end and gamma_at < h_end or rstd_at and rstd_at < h_end and h_at < r_end)):
+        _check_apart(3, (y_at, 2 * n, "y"), (h_at, 2 * n if h_at else 0, "h"), (rstd_at, 4 * rows if rstd_at else 0, "rstd"),
+                     (gamma_at, 4 * C, "gamma"), (x_at, 0 if x_at in (y_at, h_at) else 2 * n, "x"),
+                     (res_at, 0 if res_at in (0, y_at, h_at) else 2 * n, "residual"))
+    stream = _stream_of("x gamma y residual h rstd", x, gamma, y, residual, h, rstd)
     call = _RMS_FWD_CALL.pack(x_at, res_at, h_at, y_at, 0, 0, rstd_at, gamma_at, rows, C, c_valid, eps, 1 if relu else 0)
     check(_native.cuda().rb_rms_norm_fwd(call, stream), "rb_rms_norm_fwd")
 
@@ -697,15 +728,22 @@ def rms_norm_fwd(x, rows, C, c_valid, eps, gamma, y, rstd=None, residual=None, h
 def rms_norm_fwd_e4m3(x, rows, C, c_valid, eps, gamma, q, scales, residual=None, h=None, relu=False):
     """`rms_norm_fwd` with its output in 8 bits: y is about q * scales[row], q e4m3 (torch.float8_e4m3fn) and scales float32
     [rows], the largest |y| of the row / 448 (1 in a row of zeros, never below 2^-126). y is not rounded in between. A row that
-    holds a NaN or an infinity has a NaN as its scale and NaN codes. `q` overlaps no other operand; `h` may be `x` or `residual`."""
+    holds a NaN or an infinity has a NaN as its scale and NaN codes. `q` and `scales` overlap no other operand;
+    `h` may be `x` or `residual`."""
     x_at, gamma_at, res_at, h_at = _rms_inputs(x, rows, C, c_valid, eps, gamma, residual, h)
     n = rows * C
     q_at = _operand("q", q, torch.float8_e4m3fn, n)
     scales_at = _operand("scales", scales, torch.float32, rows, 4)
-    for other, at in (("x", x_at), ("residual", res_at), ("h", h_at)):
-        if at:
-            _check_apart("q", q_at, n, other, at, 2 * n, False)
-    stream = _stream_of(x=x, gamma=gamma, q=q, scales=scales, residual=residual, h=h)
+    # q, scales and h overlap nothing, except for h exactly in the place of x or residual
+    x_end, q_end, g_end, s_end, res_end, h_end = x_at + 2 * n, q_at + n, gamma_at + 4 * C, scales_at + 4 * rows, res_at + 2 * n, h_at + 2 * n
+    if (q_at < x_end and x_at < q_end or q_at < g_end and gamma_at < q_end or q_at < s_end and scales_at < q_end or
+            scales_at < x_end and x_at < s_end or scales_at < g_end and gamma_at < s_end or
+            res_at and (q_at < res_end and res_at < q_end or scales_at < res_end and res_at < s_end) or
+            h_at and (h_at < x_end and x_at < h_end and x_at != h_at or h_at < res_end and res_at < h_end and res_at != h_at or
+                      h_at < q_end and q_at < h_end or h_at < g_end and gamma_at < h_end or h_at < s_end and scales_at < h_end)):
+        _check_apart(3, (q_at, n, "q"), (scales_at, 4 * rows, "scales"), (h_at, 2 * n if h_at else 0, "h"), (gamma_at, 4 * C, "gamma"),
+                     (x_at, 0 if x_at == h_at else 2 * n, "x"), (res_at, 0 if res_at in (0, h_at) else 2 * n, "residual"))
+    stream = _stream_of("x gamma q scales residual h", x, gamma, q, scales, residual, h)
     call = _RMS_FWD_CALL.pack(x_at, res_at, h_at, 0, q_at, scales_at, 0, gamma_at, rows, C, c_valid, eps, 1 if relu else 0)
     check(_native.cuda().rb_rms_norm_fwd(call, stream), "rb_rms_norm_fwd")
 
@@ -728,20 +766,32 @@ def rms_norm_bwd(h, dy, rows, C, c_valid, rstd, gamma, dgamma, dx, ws, add=None,
     """Backward of `rms_norm_fwd`: dx = the delta of h (and so of x and of the residual), plus `add`, the delta that h has from
     elsewhere; dgamma += its sum over the rows, in the same order every time. `dy` is the delta of y; with `relu` it is masked
     here by the sign of y, which is worked out again. `h`: what was normalised (x where there was no residual). `dx` may be `h`,
-    `dy` or `add`; `ws`: `rms_norm_scratch`."""
+    `dy` or `add`; `ws`: `rms_norm_scratch`. Nothing else that is written may overlap an operand."""
     _check_rms_shape(rows, C, c_valid)
     n = rows * C
     h_at = _operand("h", h, torch.bfloat16, n)
     dy_at = _operand("dy", dy, torch.bfloat16, n)
     dx_at = _operand("dx", dx, torch.bfloat16, n)
     add_at = 0 if add is None else _operand("add", add, torch.bfloat16, n)
-    for other, at in (("h", h_at), ("dy", dy_at), ("add", add_at)):
-        if at:
-            _check_apart("dx", dx_at, 2 * n, other, at, 2 * n, True)
     rstd_at = _operand("rstd", rstd, torch.float32, rows, 4)
     gamma_at = _operand("gamma", gamma, torch.float32, C)
     dgamma_at = _operand("dgamma", dgamma, torch.float32, C)
-    ws_at = _operand("scratch", ws, torch.float32, _rms_scratch_rows(C) * C)
-    stream = _stream_of(h=h, dy=dy, dx=dx, rstd=rstd, gamma=gamma, dgamma=dgamma, scratch=ws, add=add)
+    ws_size = _rms_scratch_rows(C) * C
+    ws_at = _operand("scratch", ws, torch.float32, ws_size)
+    # dx, dgamma and the scratch overlap nothing, except for dx exactly in the place of h, dy or add
+    h_end, dy_end, add_end, dx_end, r_end = h_at + 2 * n, dy_at + 2 * n, add_at + 2 * n, dx_at + 2 * n, rstd_at + 4 * rows
+    g_end, dg_end, ws_end = gamma_at + 4 * C, dgamma_at + 4 * C, ws_at + 4 * ws_size
+    if (dx_at < h_end and h_at < dx_end and h_at != dx_at or dx_at < dy_end and dy_at < dx_end and dy_at != dx_at or
+            dx_at < g_end and gamma_at < dx_end or dx_at < r_end and rstd_at < dx_end or dx_at < dg_end and dgamma_at < dx_end or
+            dgamma_at < h_end and h_at < dg_end or dgamma_at < dy_end and dy_at < dg_end or dgamma_at < g_end and gamma_at < dg_end or
+            dgamma_at < r_end and rstd_at < dg_end or
+            ws_at < h_end and h_at < ws_end or ws_at < dy_end and dy_at < ws_end or ws_at < dx_end and dx_at < ws_end or
+            ws_at < g_end and gamma_at < ws_end or ws_at < r_end and rstd_at < ws_end or ws_at < dg_end and dgamma_at < ws_end or
+            add_at and (dx_at < add_end and add_at < dx_end and add_at != dx_at or dgamma_at < add_end and add_at < dg_end or
+                        ws_at < add_end and add_at < ws_end)):
+        _check_apart(3, (dx_at, 2 * n, "dx"), (dgamma_at, 4 * C, "dgamma"), (ws_at, 4 * ws_size, "scratch"), (gamma_at, 4 * C, "gamma"),
+                     (rstd_at, 4 * rows, "rstd"), (h_at, 0 if h_at == dx_at else 2 * n, "h"), (dy_at, 0 if dy_at == dx_at else 2 * n, "dy"),
+                     (add_at, 0 if add_at in (0, dx_at) else 2 * n, "add"))
+    stream = _stream_of("h dy dx rstd gamma dgamma scratch add", h, dy, dx, rstd, gamma, dgamma, ws, add)
     call = _RMS_BWD_CALL.pack(h_at, dy_at, add_at, dx_at, rstd_at, gamma_at, dgamma_at, ws_at, rows, C, c_valid, 1 if relu else 0, 0)
     check(_native.cuda().rb_rms_norm_bwd(call, stream), "rb_rms_norm_bwd")
