@@ -362,10 +362,9 @@ __global__ void __launch_bounds__(RmsBlock<L>::most, RmsBackBlocks<L, V>::n) rms
         sum = fma2(g, t, sum);
       }
     }
-    // dx = r g gamma - h r^2 m
+    // dx = r (g gamma - h r m): r^2 m would leave fp32 where h is large and the deltas are small
     const float m = join_row<L>(parts(sum).x + parts(sum).y, slots[turn], Plus()) * a.inv_valid;
-    const float by = -(m * rstd) * rstd;
-    const f2 by2 = both(by, by);
+    const f2 by = both(-(m * rstd), -(m * rstd));
     bf16* dx = a.dx + r0 * a.C;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -373,9 +372,8 @@ __global__ void __launch_bounds__(RmsBlock<L>::most, RmsBackBlocks<L, V>::n) rms
       Vec8 d;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const f2 gg = mul2(widen(gv[j].w[k]), w.gamma[j][k]);
-        const f2 t = ADD ? fma2(gg, rs, widen(av[j].w[k])) : mul2(gg, rs);
-        d.w[k] = to_bf16(fma2(widen(hv[j].w[k]), by2, t));
+        const f2 t = fma2(widen(hv[j].w[k]), by, mul2(widen(gv[j].w[k]), w.gamma[j][k]));
+        d.w[k] = to_bf16(ADD ? fma2(t, rs, widen(av[j].w[k])) : mul2(t, rs));
       }
       if (dead) keep_live(d, w.live[j]);
       store_vec(dx + off + w.next(j), d);
