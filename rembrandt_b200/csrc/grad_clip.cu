@@ -10,6 +10,7 @@
 // (us, and at the copy rate of 6.5 TB/s): norm of 62.4 M fp32 values 37.9 (38.2), of bf16 ones 21.6 (19.1); clipping 79 (76) and
 // 40.4 (38.2); both together 118 and 58, because about 25 MB of what the norm has read is still in the L2.
 #include "launch.cuh"
+#include "clip_factor.cuh"
 #include "common.cuh"
 #include "f32x2.cuh"
 #include <cooperative_groups.h>
@@ -220,11 +221,26 @@ __global__ void __launch_bounds__(256) grad_norm_kernel(const double* __restrict
 }
 
 template <int TYPE>
-__device__ __forceinline__ void scale_part(const Part& p, float f, bool zero) {
+__device__ __forceinline__ void scale_part(const Part& p, const ClipFactor& f, bool zero) {
   constexpr int PER = TYPE == 0 ? 4 : 8;
   uint4 v[VECTORS];
 #pragma unroll
   for (int i = 0; i < VECTORS; ++i) v[i] = load_part<TYPE>(p, i);
+  float by = f.by;
+  if (f.back != 1.f) {
+    if (TYPE == 2) by *= f.back;    // no fp16 value is large enough to matter
+#pragma unroll
+    for (int i = 0; i < VECTORS; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t& w = reinterpret_cast<uint32_t*>(&v[i])[j];
+        if (TYPE == 0) w = __float_as_uint(value<0>(v[i], j) * f.back);
+        if (TYPE == 1) {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(value<1>(v[i], 2 * j) * f.back, value<1>(v[i], 2 * j + 1) * f.back);
+          w = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+  }
 #pragma unroll
   for (int i = 0; i < VECTORS; ++i) {
     const long long n = p.v + 256 * i;
@@ -234,9 +250,9 @@ __device__ __forceinline__ void scale_part(const Part& p, float f, bool zero) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (TYPE == 0) {
-        w[j] = zero ? 0u : __float_as_uint(value<0>(v[i], j) * f);
+        w[j] = zero ? 0u : __float_as_uint(value<0>(v[i], j) * by);
       } else {
-        const float a = zero ? 0.f : value<TYPE>(v[i], 2 * j) * f, b = zero ? 0.f : value<TYPE>(v[i], 2 * j + 1) * f;
+        const float a = zero ? 0.f : value<TYPE>(v[i], 2 * j) * by, b = zero ? 0.f : value<TYPE>(v[i], 2 * j + 1) * by;
         if (TYPE == 1) {
           const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
           w[j] = *reinterpret_cast<const uint32_t*>(&h);
@@ -269,8 +285,9 @@ template <int TENSORS>
 __global__ void __launch_bounds__(256) clip_kernel(const __grid_constant__ GradTable<TENSORS> t, const float* __restrict__ out,
                                                    float scale, int run) {
   pdl_prolog();
-  const float coef = out[1], f = scale * coef;
-  if (f == 1.f) return;
+  const float coef = out[1];
+  const ClipFactor f = clip_factor(scale, coef);
+  if (f.by == 1.f) return;
   const bool zero = coef == 0.f;
   int k = blockIdx.x * run;
   const int end = min(k + run, t.chunks);

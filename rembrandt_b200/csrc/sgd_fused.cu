@@ -5,6 +5,7 @@
 //
 // The rules themselves are in sgd_rules.cuh.
 #include "launch.cuh"
+#include "clip_factor.cuh"
 #include "common.cuh"
 #include "sgd_rules.cuh"
 #include <algorithm>
@@ -28,18 +29,22 @@ __global__ void sgd_fused_kernel(const SgdArgs a) {
   SgdHyper h = a;
   if (h.lr_dev) h.lr = *h.lr_dev;
   bool drop = false;
+  float back = 1.f;      // gradients are taken times this before anything else
   if (CLIP) {
     const float coef = a.clip[1];
-    h.grad_scale *= coef;
+    const ClipFactor f = clip_factor(h.grad_scale, coef);
+    h.grad_scale = f.by;
+    back = f.back;
     drop = coef == 0.f;
   }
+  const bool put_g = a.mode == 5 ? a.phase & 2 : a.phase & 4;
   const long long n4 = a.n / 4;
   for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < n4;
        i += (long long)gridDim.x * blockDim.x) {
     float4 w = PASS ? __ldcs(reinterpret_cast<float4*>(a.w) + i) : reinterpret_cast<float4*>(a.w)[i];
     float4 g = reinterpret_cast<float4*>(a.g)[i];
     float4 v = a.v ? (PASS ? __ldcs(reinterpret_cast<float4*>(a.v) + i) : reinterpret_cast<float4*>(a.v)[i]) : make_float4(0.f, 0.f, 0.f, 0.f);
-    if (CLIP && drop) g = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (CLIP) g = drop ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(g.x * back, g.y * back, g.z * back, g.w * back);
     sgd_elem(w.x, g.x, v.x, h);
     sgd_elem(w.y, g.y, v.y, h);
     sgd_elem(w.z, g.z, v.z, h);
@@ -50,7 +55,7 @@ __global__ void sgd_fused_kernel(const SgdArgs a) {
     };
     if (a.phase & 3) put(a.w, w);
     if (a.v && (a.phase & 1)) put(a.v, v);
-    if ((a.phase & 4) || a.mode == 5) put(a.g, g);
+    if (put_g) put(a.g, g);
     if (a.w16 && (a.phase & 2)) {
       __nv_bfloat162 lo = __floats2bfloat162_rn(w.x, w.y), hi = __floats2bfloat162_rn(w.z, w.w);
       uint2 o;
@@ -63,11 +68,11 @@ __global__ void sgd_fused_kernel(const SgdArgs a) {
   // tail (n not a multiple of 4)
   for (long long i = n4 * 4 + blockIdx.x * (long long)blockDim.x + threadIdx.x; i < a.n;
        i += (long long)gridDim.x * blockDim.x) {
-    float w = a.w[i], g = CLIP && drop ? 0.f : a.g[i], v = a.v ? a.v[i] : 0.f;
+    float w = a.w[i], g = !CLIP ? a.g[i] : drop ? 0.f : a.g[i] * back, v = a.v ? a.v[i] : 0.f;
     sgd_elem(w, g, v, h);
     if (a.phase & 3) a.w[i] = w;
     if (a.v && (a.phase & 1)) a.v[i] = v;
-    if ((a.phase & 4) || a.mode == 5) a.g[i] = g;
+    if (put_g) a.g[i] = g;
     if (a.w16 && (a.phase & 2)) a.w16[i] = f2bf(w);
   }
 }
