@@ -529,7 +529,7 @@ def grad_norm(tensors, max_norm, out, ws, scale=1.0):
 
 
 def _check_scale(scale):
-    if not 2.0 ** -126 <= scale < 2.0 ** 128:
+    if not 2.0 ** -126 <= scale < 2.0 ** 128 - 2.0 ** 103:      # what rounds to an infinity is none
         raise ValueError(f"a scale of gradients has to be a positive float32, not {scale}")
 
 

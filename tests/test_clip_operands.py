@@ -149,3 +149,20 @@ def test_a_coefficient_inside_of_what_the_sweep_writes(as_on_a_gpu, where):
         _sweep(torch.zeros(2), **{where: t})
     with pytest.raises(as_on_a_gpu):          # behind what the sweep takes of it
         _sweep(floats[-2:], n=64 - 4, **{where: t})
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 128 - 2.0 ** 103, 2.0 ** 128 * (1 - 2.0 ** -30)])
+def test_scales_that_round_to_infinity(no_launch, scale):
+    assert torch.tensor(scale, dtype=torch.float32).isinf()
+    with pytest.raises(ValueError, match="scale"):
+        K.grad_norm([], 1.0, torch.zeros(2), K.grad_norm_scratch("cpu"), scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        K.clip_grads([], torch.zeros(2), scale=scale)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 128 - 2.0 ** 104, 2.0 ** -126])
+def test_the_largest_and_smallest_scale(as_on_a_gpu, scale):
+    with pytest.raises(as_on_a_gpu):
+        K.grad_norm([], 1.0, torch.zeros(2), K.grad_norm_scratch("cpu"), scale=scale)
+    with pytest.raises(as_on_a_gpu):
+        K.clip_grads([], torch.zeros(2), scale=scale)
