@@ -50,7 +50,7 @@ def base_parser(desc, **defaults):
     ap.add_argument("--keep-averaged", action="store_true",
                     help="continue from the averaged model after a checkpoint (default: every rank keeps its own)")
     ap.add_argument("--comm", default=defaults.get("comm", "auto"),
-                    help="exchange backend: auto (fused_allreduce_sgd on GPUs, allreduce on CPU ranks) | kernel backends "
+                    help="exchange backend: auto (fused_allreduce_sgd on GPUs, allreduce on CPU ranks and with --clip-norm) | kernel backends "
                          "fused_allreduce_sgd, gossip_p2p, gossip_pull_p2p, gossip_push_p2p, group_allreduce_gossip_p2p, "
                          "elastic_p2p | library backends allreduce, gossip_pair, gossip_pull, gossip_push, "
                          "group_allreduce_gossip, elastic, and on CPU ranks their asynchronous forms gossip_push_async, "
@@ -117,11 +117,12 @@ def init_distributed(device: str, args=None):
     return rank, world
 
 
-def make_comm(name, device, world):
+def make_comm(name, device, world, clip_norm=0.0):
     if world <= 1:
         return comm_mod.NullComm()
     if name == "auto":
-        name = "fused_allreduce_sgd" if device == "cuda" else "allreduce"
+        # clipping needs the norm of all gradients before the first parameter is updated
+        name = "fused_allreduce_sgd" if device == "cuda" and not clip_norm else "allreduce"
     return comm_mod.make_comm(name)
 
 
@@ -137,7 +138,7 @@ def run_training(args, model_cfg, schedule: StepSizeSchedule = None, source=None
     rank, world = init_distributed(args.device, args)
     device = torch.device(args.device, int(os.environ.get("LOCAL_RANK", "0")) if args.device == "cuda" else None) \
         if args.device == "cuda" else torch.device("cpu")
-    worker = make_comm(args.comm, args.device, world)
+    worker = make_comm(args.comm, args.device, world, args.clip_norm)
     seed = worker.broadcast_seed((args.seed, args.seed * 7919 + 13))
     dims = model_cfg.input_op.cfg.in_dims
     classes = model_cfg.loss_op.cfg.num_categories
