@@ -20,8 +20,8 @@ from .sgd import Momentum, clip_coefficient, reference_step
 
 class SgdStepper:
     def __init__(self, net, momentum: Momentum, mu: float, l2: float, clip_norm: float = 0.0):
-        if not 0.0 <= clip_norm < math.inf:
-            raise ValueError(f"gradients are clipped to a norm above 0 (0: not at all), not {clip_norm}")
+        if not (clip_norm == 0.0 or 2.0 ** -149 <= clip_norm < math.inf):
+            raise ValueError(f"gradients are clipped to a norm that is a float32 above 0 (0: not at all), not {clip_norm}")
         self.net = net
         self.mode = int(momentum)
         self.mu = float(mu) if momentum != Momentum.ZERO else 0.0
