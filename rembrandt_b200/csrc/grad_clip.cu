@@ -362,12 +362,15 @@ int rb_grad_norm(const void* list, float scale, float max_norm, float* out, doub
   int again = 0;
   bool done = false;
   const bool ok = for_tables(list, [&](const auto& t) {
-    done = !again && t.chunks <= SMALL_CHUNKS && sizeof(t.first) / 4 == FEW;
-    if (done) {
-      launch_pdl(grad_norm_small_kernel<sizeof(t.first) / 4>, CLUSTER, 1024, 0, st, t, out, (double)scale, max_norm);
-      return;
+    constexpr int TENSORS = sizeof(t.first) / sizeof(int);
+    if constexpr (TENSORS == FEW) {
+      done = !again && t.chunks <= SMALL_CHUNKS;
+      if (done) {
+        launch_pdl(grad_norm_small_kernel<FEW>, CLUSTER, 1024, 0, st, t, out, (double)scale, max_norm);
+        return;
+      }
     }
-    launch_pdl(grad_squares_kernel<sizeof(t.first) / 4>, std::min(t.chunks, NORM_BLOCKS), 256, 0, st, t, ws, again);
+    launch_pdl(grad_squares_kernel<TENSORS>, std::min(t.chunks, NORM_BLOCKS), 256, 0, st, t, ws, again);
     again = 1;
   });
   if (!ok) return -10;
