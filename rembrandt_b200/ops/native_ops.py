@@ -675,8 +675,8 @@ def _check_rms_eps(eps):
 
 
 def _check_apart(written, *spans):
-    """`spans`: (address, bytes, name) of the operands of a call that overlap, as far as a quick look can tell; those that it
-    writes are the first `written` ones. An input that one of these exactly stands in the place of is not among them."""
+    """`spans`: (address, bytes, name) of the operands of a call; those that it writes are the first `written` ones, and
+    ValueError names one that overlaps another. An input that one of these exactly stands in the place of has no bytes here."""
     for i, (at, size, name) in enumerate(spans[:written]):
         for other_at, other_size, other in spans[i + 1:]:
             if max(at, other_at) < min(at + size, other_at + other_size):
@@ -728,8 +728,8 @@ def rms_norm_fwd(x, rows, C, c_valid, eps, gamma, y, rstd=None, residual=None, h
 def rms_norm_fwd_e4m3(x, rows, C, c_valid, eps, gamma, q, scales, residual=None, h=None, relu=False):
     """`rms_norm_fwd` with its output in 8 bits: y is about q * scales[row], q e4m3 (torch.float8_e4m3fn) and scales float32
     [rows], the largest |y| of the row / 448 (1 in a row of zeros, never below 2^-126). y is not rounded in between. A row that
-    holds a NaN or an infinity has a NaN as its scale and NaN codes. `q` and `scales` overlap no other operand;
-    `h` may be `x` or `residual`."""
+    holds a NaN or an infinity has a NaN as its scale and NaN codes; one whose squares pass float32 is a row of zeros. `q` and
+    `scales` overlap no other operand; `h` may be `x` or `residual`."""
     x_at, gamma_at, res_at, h_at = _rms_inputs(x, rows, C, c_valid, eps, gamma, residual, h)
     n = rows * C
     q_at = _operand("q", q, torch.float8_e4m3fn, n)
@@ -765,7 +765,8 @@ def rms_norm_scratch(C, device):
 def rms_norm_bwd(h, dy, rows, C, c_valid, rstd, gamma, dgamma, dx, ws, add=None, relu=False):
     """Backward of `rms_norm_fwd`: dx = the delta of h (and so of x and of the residual), plus `add`, the delta that h has from
     elsewhere; dgamma += its sum over the rows, in the same order every time. `dy` is the delta of y; with `relu` it is masked
-    here by the sign of y, which is worked out again. `h`: what was normalised (x where there was no residual). `dx` may be `h`,
+    here by the sign of y, which is worked out again. `h`: what was normalised (x where there was no residual). A row
+    whose factor is 0, because its squares pass float32, adds nothing to `dgamma` and its dx is `add`. `dx` may be `h`,
     `dy` or `add`; `ws`: `rms_norm_scratch`. Nothing else that is written may overlap an operand."""
     _check_rms_shape(rows, C, c_valid)
     n = rows * C

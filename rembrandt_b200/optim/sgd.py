@@ -162,13 +162,15 @@ class SgdOptConfig:
     valid_iters: int = 0
     checkpoint_dir: Optional[str] = None
     max_iters: int = 0
-    clip_norm: float = 0.0             # largest global norm of an iteration's gradients; 0 = they are taken as they are
+    clip_norm: float = 0.0             # largest global norm of an iteration's gradients; 0 = they are taken as they are.
+                                       # GRAD_DECAY: of the gradient buffer, in which the momentum is
 
 
 # ------------------------------------------------------------------------------------------ rules
 def clip_coefficient(norm: float, max_norm: float) -> float:
     """The factor that brings gradients of this global norm down to `max_norm`: 1 where they are within it, 0 where the norm is
-    not finite (the step is then one with gradients of zeros). It multiplies the loss's gradients, before the L2 term."""
+    not finite (the step is then one with gradients of zeros). It multiplies the loss's gradients, before the L2 term; with
+    GRAD_DECAY all that the gradient buffer holds, which is mu times the last step's gradients and L2 term besides."""
     if not math.isfinite(norm):
         return 0.0
     return max_norm / norm if norm > max_norm else 1.0

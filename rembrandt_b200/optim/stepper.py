@@ -6,7 +6,8 @@ once for the unregularised tail; on CPU it is ``reference_step``. ``phase`` lets
 the two (the reference's SyncParamsThenStep order, src/opt/sgd/new.rs:408-431).
 
 With `clip_norm` the gradients of all parameters are measured first (csrc/grad_clip.cu) and the sweep multiplies them by the
-coefficient, which it reads on the device: a captured step clips as an eager one does.
+coefficient, which it reads on the device: a captured step clips as an eager one does. What is measured is the gradient buffer:
+with the rule that keeps its momentum there (GRAD_DECAY), the momentum is part of the norm and is clipped with the rest.
 """
 from __future__ import annotations
 
