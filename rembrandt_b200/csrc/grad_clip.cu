@@ -220,27 +220,14 @@ __global__ void __launch_bounds__(256) grad_norm_kernel(const double* __restrict
   if (threadIdx.x == 0) put_norm(s, scale, max_norm, out);
 }
 
-template <int TYPE>
+template <int TYPE, bool LOW>
 __device__ __forceinline__ void scale_part(const Part& p, const ClipFactor& f, bool zero) {
   constexpr int PER = TYPE == 0 ? 4 : 8;
   uint4 v[VECTORS];
 #pragma unroll
   for (int i = 0; i < VECTORS; ++i) v[i] = load_part<TYPE>(p, i);
-  float by = f.by;
-  if (f.back != 1.f) {
-    if (TYPE == 2) by *= f.back;    // no fp16 value is large enough to matter
-#pragma unroll
-    for (int i = 0; i < VECTORS; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t& w = reinterpret_cast<uint32_t*>(&v[i])[j];
-        if (TYPE == 0) w = __float_as_uint(value<0>(v[i], j) * f.back);
-        if (TYPE == 1) {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(value<1>(v[i], 2 * j) * f.back, value<1>(v[i], 2 * j + 1) * f.back);
-          w = *reinterpret_cast<const uint32_t*>(&h);
-        }
-      }
-  }
+  // value j of a vector, times the factor
+  auto scaled = [&](const uint4& vec, int j) { return zero ? 0.f : LOW ? value<TYPE>(vec, j) * f.back * f.by : value<TYPE>(vec, j) * f.by; };
 #pragma unroll
   for (int i = 0; i < VECTORS; ++i) {
     const long long n = p.v + 256 * i;
@@ -250,9 +237,9 @@ __device__ __forceinline__ void scale_part(const Part& p, const ClipFactor& f, b
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (TYPE == 0) {
-        w[j] = zero ? 0u : __float_as_uint(value<0>(v[i], j) * by);
+        w[j] = __float_as_uint(scaled(v[i], j));
       } else {
-        const float a = zero ? 0.f : value<TYPE>(v[i], 2 * j) * by, b = zero ? 0.f : value<TYPE>(v[i], 2 * j + 1) * by;
+        const float a = scaled(v[i], 2 * j), b = scaled(v[i], 2 * j + 1);
         if (TYPE == 1) {
           const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
           w[j] = *reinterpret_cast<const uint32_t*>(&h);
@@ -281,6 +268,19 @@ __device__ __forceinline__ void scale_part(const Part& p, const ClipFactor& f, b
 // clip, and the longer it takes them to find that there is nothing to do (62.4 M fp32 values, us for one and for the other: 888 blocks
 // 87.6 and 1.3, 1776 83.3 and 2.2, 3552 79.1 and 3.7, 8000 75.8 and 8.3, one a chunk 74.4 and 16.2).
 constexpr int CLIP_BLOCKS = 3552;
+template <bool LOW, int TENSORS>
+__device__ __forceinline__ void clip_run(const GradTable<TENSORS>& t, const ClipFactor& f, bool zero, int run) {
+  int k = blockIdx.x * run;
+  const int end = min(k + run, t.chunks);
+  for (int i = tensor_of(t, k); k < end; ++k) {
+    while (i + 1 < t.count && t.first[i + 1] <= k) ++i;
+    const Part p = part_of(t, i, k, threadIdx.x);
+    if (p.type == 0) scale_part<0, LOW>(p, f, zero);
+    else if (p.type == 1) scale_part<1, LOW>(p, f, zero);
+    else scale_part<2, LOW>(p, f, zero);
+  }
+}
+
 template <int TENSORS>
 __global__ void __launch_bounds__(256) clip_kernel(const __grid_constant__ GradTable<TENSORS> t, const float* __restrict__ out,
                                                    float scale, int run) {
@@ -288,16 +288,8 @@ __global__ void __launch_bounds__(256) clip_kernel(const __grid_constant__ GradT
   const float coef = out[1];
   const ClipFactor f = clip_factor(scale, coef);
   if (f.by == 1.f) return;
-  const bool zero = coef == 0.f;
-  int k = blockIdx.x * run;
-  const int end = min(k + run, t.chunks);
-  for (int i = tensor_of(t, k); k < end; ++k) {
-    while (i + 1 < t.count && t.first[i + 1] <= k) ++i;
-    const Part p = part_of(t, i, k, threadIdx.x);
-    if (p.type == 0) scale_part<0>(p, f, zero);
-    else if (p.type == 1) scale_part<1>(p, f, zero);
-    else scale_part<2>(p, f, zero);
-  }
+  if (f.back == 1.f) clip_run<false>(t, f, false, run);
+  else clip_run<true>(t, f, coef == 0.f, run);
 }
 
 }  // namespace rb

@@ -399,7 +399,7 @@ def sgd_fused(w, g, v, w16, n, lr, mu, l2, grad_scale, mode, phase=7, clip=None)
         end, reach = clip_at + 8, clip_at - 4 * n
         if (reach < w_at < end or reach < g_at < end or v_at and reach < v_at < end or w16_at and clip_at - 2 * n < w16_at < end):
             raise ValueError("clip overlaps what the sweep writes")
-        stream = _stream_of("clip w g v w16", clip, w, g, v, w16)
+        stream = _stream_of("clip w g", clip, w, g)
     check(_native.cuda().rb_sgd_fused(w_at, g_at, v_at, w16_at, n, *rate_args(lr), mu, l2, grad_scale, mode, phase, clip_at,
                                       stream), "rb_sgd_fused")
 
